@@ -172,6 +172,133 @@ llx_status llx_tp_init(llx_model* m, const void* id, int rank, int world);
 llx_status llx_linear_argmax_noalloc(const int8_t* A, const int8_t* W, const int32_t* bias, const int32_t* rq, int R,
                                      int N, int K, int vocab, int16_t* logits, int32_t* argmax, void* stream);
 
+/* ---- Paged serving: ragged launches over a paged int8 KV cache, and sampled tokens ----------
+ * No counterpart in the reference, which runs one sequence over a dense cache; the arithmetic
+ * is the reference's (norms, rotation, requantization, attention: docs/NUMERICS.md), bit for
+ * bit, whatever the pages, the chunking or the batch.
+ *
+ * Cache of a layer: k and v [n_pages][n_kv_heads][page_size][head_dim] int8 (the last three
+ * axes dense, pages page_stride bytes apart).  Position t of the sequence in slot s lies in
+ * page table[s][t / page_size], row t % page_size.  length[s] counts its positions.
+ * A launch's rows: sequence i of n_seqs sits in slot seqs[i] (seqs null: slot i) and brings the
+ * rows q_start[i] <= r < q_start[i + 1], its newest positions: row r is at position
+ * length[slot] - (q_start[i + 1] - r).  Rows behind q_start[n_seqs] are left as they were.
+ *
+ * Tables, lengths and row starts are device memory, read by the kernels: the calls only
+ * enqueue on `stream` (a cudaStream_t, null: default stream) and can be captured.  What the
+ * device finds wrong with them is skipped, never accessed, and ORed into *status (device
+ * memory, may be null); what the host can see is refused with an error code.  `device` is the
+ * CUDA device of the pointers and of the stream; the caller's current device is left as it was.
+ * Every field is 8 bytes wide. */
+#define LLX_STATUS_BAD_PAGE 1      /* a position whose page id is outside the cache */
+#define LLX_STATUS_BAD_POSITION 2  /* a position below 0, or beyond the rotation or page tables */
+#define LLX_STATUS_BAD_BOUND 4     /* a sequence with more rows or positions than the call was told */
+#define LLX_STATUS_NO_PAGES 8      /* too few free pages: nothing was changed */
+#define LLX_STATUS_BAD_SLOT 16     /* a slot outside the table, listed twice, or both parent and child */
+#define LLX_STATUS_SHARED_PAGE 32  /* new positions would fall into a page that others share */
+
+/* q [rows][n_heads][head_dim], k [rows][n_kv_heads][head_dim] i16 and v (i8) of the launch: norm
+ * of every query and key head (gamma null: none), rotation (cos / sin [n_positions][head_dim / 2]
+ * Q1.14), requantization to i8 (M, S); q8 [rows][n_heads][head_dim] is written, keys and values
+ * go to their pages.  Strides are in elements between rows. A row without a place in the cache
+ * (see status) gets zeros in q8 and writes no page. */
+typedef struct {
+  const int16_t *q, *k;
+  const int8_t* v;
+  int8_t* q8;
+  int64_t q_stride, k_stride, v_stride, q8_stride;
+  int64_t rows, n_heads, n_kv_heads, head_dim;
+  const int16_t *q_gamma, *k_gamma;
+  int64_t q_eps, q_C, q_shift, k_eps, k_C, k_shift;
+  const int16_t *cos, *sin;
+  int64_t n_positions;
+  int64_t q_M, q_S, k_M, k_S;
+  int8_t *k_pages, *v_pages;
+  int64_t page_stride, n_pages, page_size;
+  const int32_t* table;
+  int64_t table_stride, max_seqs, max_pages;
+  const int32_t *length, *q_start, *seqs;
+  int64_t n_seqs;
+  int32_t* status;
+  int64_t device;
+} llx_paged_append_args;
+llx_status llx_paged_append(const llx_paged_append_args* a, void* stream);
+
+/* Causal attention of the launch's rows over their sequences' pages: q8 -> out, both
+ * [rows][n_heads][head_dim] i8 (16-byte aligned rows).  score: z = mulshift(max - s, Ms, Ss),
+ * output: mulshift(o, Mo, So), prob_bits 8 or 15.  Keys whose page id is outside the cache count
+ * as absent; a row without keys gets zeros.  max_rows and max_len bound every sequence's rows and
+ * length (they size the launch; rows and positions beyond them are not computed). */
+typedef struct {
+  const int8_t* q8;
+  int8_t* out;
+  int64_t q8_stride, out_stride;
+  int64_t rows, n_heads, n_kv_heads, head_dim;
+  const int8_t *k_pages, *v_pages;
+  int64_t page_stride, n_pages, page_size;
+  const int32_t* table;
+  int64_t table_stride, max_seqs, max_pages;
+  const int32_t *length, *q_start, *seqs;
+  int64_t n_seqs, max_rows, max_len;
+  int64_t Ms, Ss, Mo, So, prob_bits;
+  int32_t* status;
+  int64_t device;
+} llx_paged_attention_args;
+llx_status llx_paged_attention(const llx_paged_attention_args* a, void* stream);
+
+/* Page management.  refs[page] counts the table entries that name it (0: free); new pages are
+ * the free ones with the lowest ids.  k and v hold n_layers layers, layer_stride bytes apart.
+ *   reserve: list_a = slots, list_b = new positions per slot; length grows by them and the pages
+ *            they need are taken.  All or nothing.
+ *   fork:    list_a = parents, list_b = children.  A child's old pages are released, then it
+ *            becomes its parent's copy: with share, full pages are shared and a part-filled last
+ *            page is copied; without, every page is copied.  Rows past the parent's length are
+ *            not copied.  A child may be listed once and may not be a parent.  All or nothing.
+ *   free:    list_a = slots; their pages are released, their lengths set to 0.
+ *   compact: live pages move to the lowest ids, in order; new_table / new_refs receive the
+ *            renamed table (same strides as table) and counts, and may be table and refs.
+ * scratch: llx_pages_scratch(n_pages) bytes of device memory, used until the call's work is done. */
+typedef struct {
+  int8_t *k, *v;
+  int64_t layer_stride, page_stride;
+  int64_t n_layers, n_pages, n_kv_heads, page_size, head_dim;
+  int32_t* table;
+  int64_t table_stride, max_seqs, max_pages;
+  int32_t *length, *refs;
+  const int32_t *list_a, *list_b;
+  int64_t n, share;
+  int32_t *new_table, *new_refs;
+  int32_t *scratch, *status;
+  int64_t device;
+} llx_pages_args;
+size_t llx_pages_scratch(int64_t n_pages);
+llx_status llx_pages_reserve(const llx_pages_args* a, void* stream);
+llx_status llx_pages_fork(const llx_pages_args* a, void* stream);
+llx_status llx_pages_free(const llx_pages_args* a, void* stream);
+llx_status llx_pages_compact(const llx_pages_args* a, void* stream);
+
+/* One token per row of logits [rows][>= vocab] i16 (row stride logits_stride, exponent E: a
+ * logit's value is l * 2^exponent) from given random numbers in [0, 1).  All integer: the weight
+ * of a token g steps below its row's largest is w(g), 2^31 * exp(-g * 2^exponent / temperature)
+ * to about 21 bits (kernels_sample.cu has the steps), so tokens do not depend on how the row is
+ * split over threads.  Ordered by logit, ties by index, the tokens kept are the shortest of: the
+ * first top_k (<= 0: all); of those, the shortest run whose weight reaches top_p of theirs
+ * (>= 1: all); those of weight at least min_p times the largest.  The token is the first, by
+ * index, whose running kept weight exceeds random times the whole.  temperature <= 0 or NaN: the
+ * largest logit, lowest index.  Per-row device arrays; temperature, top_k, top_p, min_p may be
+ * null (1, all, 1, 0).  prob (may be null): the token's share of the kept weight. */
+typedef struct {
+  const int16_t* logits;
+  int64_t logits_stride, rows, vocab, exponent;
+  const float *temperature, *top_p, *min_p;
+  const int32_t* top_k;
+  const double* random;
+  int32_t* token;
+  float* prob;
+  int64_t device;
+} llx_sample_args;
+llx_status llx_sample(const llx_sample_args* a, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

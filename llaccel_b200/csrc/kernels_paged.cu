@@ -1,0 +1,436 @@
+// Paged cache kernels: the launch's queries, keys and values on their way into the cache
+// (k_paged_append), and the management of pages (reserve, fork, free, compact).
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "launch.cuh"
+#include "numerics.cuh"
+#include "paged.h"
+
+namespace llx {
+
+// ---------------------------------------------------------------------------------------
+// Append: per row and head, RMSNorm over the head (numerics.h:60-71), rotation at the row's
+// position (numerics.h:75-84) and requantization; queries to q8, keys and values to the page
+// of their position.  One block per row, one warp per head at a time.
+// ---------------------------------------------------------------------------------------
+__global__ void __launch_bounds__(256) k_paged_append(const llx_paged_append_args a) {
+  pdl_trigger();
+  pdl_wait();
+  const int r = blockIdx.x;
+  const int i = find_sequence(a.q_start, (int)a.n_seqs, r);
+  if (i < 0) return;
+  const int slot = a.seqs ? a.seqs[i] : i;
+  const int D = (int)a.head_dim, half = D / 2, H = (int)a.n_heads, Hkv = (int)a.n_kv_heads;
+  int64_t pos = -1;
+  int page = -1, code = 0;
+  if (slot < 0 || slot >= a.max_seqs) {
+    code = LLX_STATUS_BAD_SLOT;
+  } else {
+    pos = (int64_t)a.length[slot] - (a.q_start[i + 1] - r);
+    if (pos < 0 || pos >= a.n_positions || pos >= a.max_pages * a.page_size) {
+      code = LLX_STATUS_BAD_POSITION;
+    } else {
+      page = a.table[slot * a.table_stride + pos / a.page_size];
+      if (page < 0 || page >= a.n_pages) code = LLX_STATUS_BAD_PAGE;
+    }
+  }
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  int8_t* q8 = a.q8 + r * a.q8_stride;
+  if (code) {
+    if (threadIdx.x == 0) raise_status(a.status, code);
+    for (int e = threadIdx.x; e < H * D; e += blockDim.x) q8[e] = 0;
+    return;
+  }
+  const int row = (int)(pos % a.page_size);
+  const int64_t head0 = (int64_t)page * a.page_stride + (int64_t)row * D;  // key / value row of head 0
+  const int64_t head_step = a.page_size * D;
+  const int16_t* ct = a.cos + pos * half;
+  const int16_t* sn = a.sin + pos * half;
+  for (int h = warp; h < H + Hkv; h += warps) {
+    const bool is_q = h < H;
+    const int hh = is_q ? h : h - H;
+    const int16_t* x = is_q ? a.q + r * a.q_stride + (int64_t)hh * D : a.k + r * a.k_stride + (int64_t)hh * D;
+    const int16_t* gamma = is_q ? a.q_gamma : a.k_gamma;
+    int64_t inv = 0;
+    if (gamma) {
+      uint64_t ss = 0;
+      for (int e = lane; e < D; e += 32) ss += (uint64_t)((int64_t)x[e] * x[e]);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      const uint32_t root = isqrt48_fast(ss + (uint64_t)(is_q ? a.q_eps : a.k_eps));
+      const uint64_t v = udiv_fast((uint64_t)(is_q ? a.q_C : a.k_C), root ? root : 1);
+      inv = v < 65535 ? (int64_t)v : 65535;
+    }
+    const int sh = (int)(is_q ? a.q_shift : a.k_shift);
+    const int64_t M = is_q ? a.q_M : a.k_M;
+    const int S = (int)(is_q ? a.q_S : a.k_S);
+    int8_t* dst = is_q ? q8 + (int64_t)hh * D : a.k_pages + head0 + hh * head_step;
+    for (int e = lane; e < half; e += 32) {
+      int64_t x1 = x[e], x2 = x[e + half];
+      if (gamma) {
+        x1 = sat16(rshr(x1 * gamma[e] * inv, sh));
+        x2 = sat16(rshr(x2 * gamma[e + half] * inv, sh));
+      }
+      const int64_t c = ct[e], s = sn[e];
+      dst[e] = (int8_t)sat8(mulshift(sat16(rshr(x1 * c - x2 * s, 14)), M, S));
+      dst[e + half] = (int8_t)sat8(mulshift(sat16(rshr(x2 * c + x1 * s, 14)), M, S));
+    }
+  }
+  const int8_t* v = a.v + r * a.v_stride;
+  for (int e = threadIdx.x; e < Hkv * D; e += blockDim.x) a.v_pages[head0 + (e / D) * head_step + e % D] = v[e];
+}
+
+cudaError_t launch_paged_append(const llx_paged_append_args& a, cudaStream_t st) {
+  if (a.rows == 0 || a.n_seqs == 0) return cudaSuccess;
+  return launch_k(k_paged_append, dim3((unsigned)a.rows), dim3(256), 0, st, a);
+}
+
+// ---------------------------------------------------------------------------------------
+// Page management.  One block plans (checks, counts, renames; a few thousand integers), then
+// a grid copies the pages' rows.  Whatever the order of threads, the result is the same: new
+// pages are the lowest free ids, handed out in the order of the lists.
+// ---------------------------------------------------------------------------------------
+constexpr int kPlanThreads = 1024;
+constexpr int kMaxSlots = 1 << 18;  // slots of a table (bitmap of 32 KB)
+
+// exclusive sum over the block; *total gets the whole
+__device__ int block_scan(int v, int* total) {
+  __shared__ int part[kPlanThreads / 32];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  int x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();  // part may still be read by an earlier call
+  if (lane == 31) part[w] = x;
+  __syncthreads();
+  if (w == 0) {
+    int y = part[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int z = __shfl_up_sync(0xffffffffu, y, o);
+      if (lane >= o) y += z;
+    }
+    part[lane] = y;
+  }
+  __syncthreads();
+  *total = part[kPlanThreads / 32 - 1];
+  return x - v + (w ? part[w - 1] : 0);
+}
+
+__device__ __forceinline__ int64_t pages_for(int64_t len, int64_t P) { return (len + P - 1) / P; }
+
+// positions of a slot as the table can hold them
+__device__ __forceinline__ int64_t slot_length(const llx_pages_args& a, int slot) {
+  const int64_t len = a.length[slot];
+  return len < 0 ? 0 : (len > a.max_pages * a.page_size ? a.max_pages * a.page_size : len);
+}
+
+// The lists name slots of the table, each at most once in `once` (and, for a fork, none of
+// them among `others`): checked with a bitmap of the slots.
+__device__ bool lists_fine(const llx_pages_args& a, const int32_t* once, const int32_t* others) {
+  __shared__ uint32_t seen[kMaxSlots / 32];
+  __shared__ int bad;
+  const int words = (int)((a.max_seqs + 31) / 32);
+  for (int w = threadIdx.x; w < words; w += blockDim.x) seen[w] = 0;
+  if (threadIdx.x == 0) bad = 0;
+  __syncthreads();
+  for (int64_t i = threadIdx.x; i < a.n; i += blockDim.x) {
+    const int s = once[i];
+    if (s < 0 || s >= a.max_seqs || (atomicOr(&seen[s >> 5], 1u << (s & 31)) >> (s & 31)) & 1u) bad = 1;
+  }
+  __syncthreads();
+  if (others)
+    for (int64_t i = threadIdx.x; i < a.n; i += blockDim.x) {
+      const int s = others[i];
+      if (s < 0 || s >= a.max_seqs || (seen[s >> 5] >> (s & 31)) & 1u) bad = 1;
+    }
+  __syncthreads();
+  return bad == 0;
+}
+
+// Releases (sign -1) or takes back (+1) every page of the listed slots; the entries stay.
+__device__ void count_pages(const llx_pages_args& a, const int32_t* slots, int sign) {
+  const int64_t total = a.n * a.max_pages;
+  for (int64_t x = threadIdx.x; x < total; x += blockDim.x) {
+    const int id = a.table[slots[x / a.max_pages] * a.table_stride + x % a.max_pages];
+    if (id >= 0 && id < a.n_pages) atomicAdd(&a.refs[id], sign);
+  }
+  __syncthreads();
+}
+
+// Writes the ids of the `need` lowest free pages to scratch; false if there are fewer.
+__device__ bool take_free(const llx_pages_args& a, int64_t need) {
+  const int64_t per = (a.n_pages + kPlanThreads - 1) / kPlanThreads;
+  const int64_t p0 = threadIdx.x * per, p1 = p0 + per < a.n_pages ? p0 + per : a.n_pages;
+  int mine = 0, have;
+  for (int64_t p = p0; p < p1; ++p) mine += a.refs[p] <= 0;
+  int at = block_scan(mine, &have);
+  if (have < need) return false;
+  for (int64_t p = p0; p < p1 && at < need; ++p)
+    if (a.refs[p] <= 0) a.scratch[at++] = (int32_t)p;
+  __syncthreads();
+  return true;
+}
+
+__global__ void __launch_bounds__(kPlanThreads) k_pages_reserve(const llx_pages_args a) {
+  pdl_trigger();
+  pdl_wait();
+  __shared__ int code;
+  if (threadIdx.x == 0) code = 0;
+  __syncthreads();
+  if (!lists_fine(a, a.list_a, nullptr)) {
+    if (threadIdx.x == 0) raise_status(a.status, LLX_STATUS_BAD_SLOT);
+    return;
+  }
+  const int64_t P = a.page_size;
+  int64_t need = 0;
+  for (int64_t i0 = 0; i0 < a.n; i0 += kPlanThreads) {
+    const int64_t i = i0 + threadIdx.x;
+    int mine = 0, sum;
+    if (i < a.n) {
+      const int s = a.list_a[i];
+      const int64_t len = a.length[s], more = a.list_b[i];
+      if (len < 0 || more < 0 || len + more > a.max_pages * P) {
+        atomicOr(&code, LLX_STATUS_BAD_POSITION);
+      } else {
+        mine = (int)(pages_for(len + more, P) - pages_for(len, P));
+        if (more && len % P) {
+          const int id = a.table[s * a.table_stride + len / P];
+          if (id < 0 || id >= a.n_pages) atomicOr(&code, LLX_STATUS_BAD_PAGE);
+          else if (a.refs[id] > 1) atomicOr(&code, LLX_STATUS_SHARED_PAGE);
+        }
+      }
+    }
+    block_scan(mine, &sum);
+    need += sum;
+  }
+  __syncthreads();
+  if (code || !take_free(a, need)) {
+    if (threadIdx.x == 0) raise_status(a.status, code ? code : LLX_STATUS_NO_PAGES);
+    return;
+  }
+  int64_t base = 0;
+  for (int64_t i0 = 0; i0 < a.n; i0 += kPlanThreads) {
+    const int64_t i = i0 + threadIdx.x;
+    int s = 0, mine = 0, sum;
+    int64_t len = 0;
+    if (i < a.n) {
+      s = a.list_a[i];
+      len = a.length[s];
+      mine = (int)(pages_for(len + a.list_b[i], P) - pages_for(len, P));
+    }
+    const int64_t at = base + block_scan(mine, &sum);
+    for (int j = 0; j < mine; ++j) {
+      const int id = a.scratch[at + j];
+      a.table[s * a.table_stride + pages_for(len, P) + j] = id;
+      a.refs[id] = 1;
+    }
+    if (i < a.n) a.length[s] = (int32_t)(len + a.list_b[i]);
+    base += sum;
+  }
+}
+
+__global__ void __launch_bounds__(kPlanThreads) k_pages_free(const llx_pages_args a) {
+  pdl_trigger();
+  pdl_wait();
+  const int64_t total = a.n * a.max_pages;
+  for (int64_t x = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; x < total; x += (int64_t)gridDim.x * blockDim.x) {
+    const int s = a.list_a[x / a.max_pages];
+    if (s < 0 || s >= a.max_seqs) {
+      raise_status(a.status, LLX_STATUS_BAD_SLOT);
+      continue;
+    }
+    // a slot listed twice still gives each page back once
+    const int id = atomicExch(&a.table[s * a.table_stride + x % a.max_pages], -1);
+    if (id >= 0 && id < a.n_pages) atomicSub(&a.refs[id], 1);
+    a.length[s] = 0;
+  }
+}
+
+// children become copies of their parents; the copying itself is k_pages_fork_copy's
+__global__ void __launch_bounds__(kPlanThreads) k_pages_fork(const llx_pages_args a) {
+  pdl_trigger();
+  pdl_wait();
+  // scratch[n_pages]: whether the copying kernel has anything to do
+  int32_t* done = a.scratch + a.n_pages;
+  if (!lists_fine(a, a.list_b, a.list_a)) {
+    if (threadIdx.x == 0) {
+      raise_status(a.status, LLX_STATUS_BAD_SLOT);
+      *done = 0;
+    }
+    return;
+  }
+  const int64_t P = a.page_size;
+  count_pages(a, a.list_b, -1);
+  int64_t need = 0;
+  for (int64_t i0 = 0; i0 < a.n; i0 += kPlanThreads) {
+    const int64_t i = i0 + threadIdx.x;
+    int mine = 0, sum;
+    if (i < a.n) {
+      const int64_t len = slot_length(a, a.list_a[i]);
+      mine = (int)(pages_for(len, P) - (a.share ? len / P : 0));
+    }
+    block_scan(mine, &sum);
+    need += sum;
+  }
+  if (!take_free(a, need)) {
+    count_pages(a, a.list_b, 1);
+    if (threadIdx.x == 0) {
+      raise_status(a.status, LLX_STATUS_NO_PAGES);
+      *done = 0;
+    }
+    return;
+  }
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  __shared__ int first[kPlanThreads];
+  int64_t base = 0;
+  for (int64_t i0 = 0; i0 < a.n; i0 += kPlanThreads) {
+    const int64_t i = i0 + threadIdx.x;
+    int mine = 0, sum;
+    if (i < a.n) {
+      const int64_t len = slot_length(a, a.list_a[i]);
+      mine = (int)(pages_for(len, P) - (a.share ? len / P : 0));
+    }
+    first[threadIdx.x] = block_scan(mine, &sum);
+    __syncthreads();
+    for (int64_t x = warp; x < kPlanThreads && i0 + x < a.n; x += kPlanThreads / 32) {
+      const int from = a.list_a[i0 + x], to = a.list_b[i0 + x];
+      const int64_t len = slot_length(a, from), held = pages_for(len, P), kept = a.share ? len / P : 0;
+      for (int64_t j = lane; j < a.max_pages; j += 32) {
+        int id = -1;
+        if (j < kept) {
+          id = a.table[from * a.table_stride + j];
+          if (id >= 0 && id < a.n_pages) atomicAdd(&a.refs[id], 1);
+        } else if (j < held) {
+          id = a.scratch[base + first[x] + j - kept];
+          a.refs[id] = 1;
+        }
+        a.table[to * a.table_stride + j] = id;
+      }
+      if (lane == 0) a.length[to] = (int32_t)len;
+    }
+    base += sum;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) *done = 1;
+}
+
+// units of (pair, page, layer, k or v): the rows that the parent has written, head by head
+__global__ void __launch_bounds__(256) k_pages_fork_copy(const llx_pages_args a) {
+  pdl_trigger();
+  pdl_wait();
+  if (!a.scratch[a.n_pages]) return;
+  const int64_t P = a.page_size, D = a.head_dim;
+  const int64_t units = a.n * a.max_pages * a.n_layers * 2;
+  for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
+    const int kv = (int)(u & 1);
+    int64_t x = u >> 1;
+    const int64_t layer = x % a.n_layers;
+    x /= a.n_layers;
+    const int64_t j = x % a.max_pages;
+    const int from = a.list_a[x / a.max_pages], to = a.list_b[x / a.max_pages];
+    const int64_t left = slot_length(a, from) - j * P;
+    if (left <= 0 || (a.share && left >= P)) continue;
+    const int src = a.table[from * a.table_stride + j], dst = a.table[to * a.table_stride + j];
+    if (src < 0 || src >= a.n_pages) {
+      if (threadIdx.x == 0) raise_status(a.status, LLX_STATUS_BAD_PAGE);
+      continue;
+    }
+    int8_t* pool = (kv ? a.v : a.k) + layer * a.layer_stride;
+    const int vecs = (int)((left < P ? left : P) * D / 16);
+    for (int h = 0; h < a.n_kv_heads; ++h) {
+      const uint4* s = reinterpret_cast<const uint4*>(pool + src * a.page_stride + h * P * D);
+      uint4* d = reinterpret_cast<uint4*>(pool + dst * a.page_stride + h * P * D);
+      for (int e = threadIdx.x; e < vecs; e += blockDim.x) d[e] = s[e];
+    }
+  }
+}
+
+// scratch: [0, N) new id of each page, [N, 2N) holes then sources of the moves, [2N, 3N) their
+// targets, [3N] number of moves
+__global__ void __launch_bounds__(kPlanThreads) k_pages_compact(const llx_pages_args a) {
+  pdl_trigger();
+  pdl_wait();
+  const int64_t N = a.n_pages, per = (N + kPlanThreads - 1) / kPlanThreads;
+  const int64_t p0 = min(N, threadIdx.x * per), p1 = min(N, p0 + per);
+  int32_t *to = a.scratch, *src = to + N, *dst = src + N;
+  int used = 0, live, moves, holes_total;
+  for (int64_t p = p0; p < p1; ++p) used += a.refs[p] > 0;
+  block_scan(used, &live);
+  // movers: live pages from id `live` on; holes: free pages below it; as many of each
+  int movers = 0, holes = 0;
+  for (int64_t p = p0; p < p1; ++p) {
+    movers += a.refs[p] > 0 && p >= live;
+    holes += a.refs[p] <= 0 && p < live;
+  }
+  int m = block_scan(movers, &moves), h = block_scan(holes, &holes_total);
+  for (int64_t p = p0; p < p1; ++p) {
+    if (a.refs[p] <= 0 && p < live) dst[h++] = (int32_t)p;
+    if (a.refs[p] > 0 && p >= live) src[m++] = (int32_t)p;
+    to[p] = (int32_t)p;
+  }
+  __syncthreads();
+  for (int x = threadIdx.x; x < moves; x += blockDim.x) to[src[x]] = dst[x];
+  // counts: every page reads its old count before any is written (new_refs may be refs)
+  for (int x = threadIdx.x; x < moves; x += blockDim.x) a.new_refs[dst[x]] = a.refs[src[x]];
+  for (int64_t p = p0; p < p1; ++p)
+    if (a.refs[p] > 0 && p < live && to[p] == p) a.new_refs[p] = a.refs[p];
+  __syncthreads();
+  for (int64_t p = live + threadIdx.x; p < N; p += blockDim.x) a.new_refs[p] = 0;
+  if (threadIdx.x == 0) to[3 * N] = moves;
+}
+
+__global__ void __launch_bounds__(256) k_pages_compact_move(const llx_pages_args a) {
+  pdl_trigger();
+  pdl_wait();
+  const int64_t N = a.n_pages;
+  const int32_t *to = a.scratch, *src = to + N, *dst = src + N;
+  const int64_t entries = a.max_seqs * a.max_pages;
+  for (int64_t x = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; x < entries; x += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t at = x / a.max_pages * a.table_stride + x % a.max_pages;
+    const int id = a.table[at];
+    a.new_table[at] = id >= 0 && id < N ? to[id] : id;
+  }
+  const int64_t units = (int64_t)to[3 * N] * a.n_layers * 2;
+  const int vecs = (int)(a.n_kv_heads * a.page_size * a.head_dim / 16);
+  for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
+    const int64_t x = u >> 1, layer = x % a.n_layers, m = x / a.n_layers;
+    int8_t* pool = ((u & 1) ? a.v : a.k) + layer * a.layer_stride;
+    const uint4* s = reinterpret_cast<const uint4*>(pool + src[m] * a.page_stride);
+    uint4* d = reinterpret_cast<uint4*>(pool + dst[m] * a.page_stride);
+    for (int e = threadIdx.x; e < vecs; e += blockDim.x) d[e] = s[e];
+  }
+}
+
+static unsigned copy_grid(int64_t units) { return (unsigned)(units < 1 ? 1 : units > 148 * 8 ? 148 * 8 : units); }
+
+cudaError_t launch_pages_reserve(const llx_pages_args& a, cudaStream_t st) {
+  if (a.n == 0) return cudaSuccess;
+  return launch_k(k_pages_reserve, dim3(1), dim3(kPlanThreads), 0, st, a);
+}
+
+cudaError_t launch_pages_free(const llx_pages_args& a, cudaStream_t st) {
+  if (a.n == 0) return cudaSuccess;
+  const int64_t blocks = (a.n * a.max_pages + kPlanThreads - 1) / kPlanThreads;
+  return launch_k(k_pages_free, dim3(copy_grid(blocks)), dim3(kPlanThreads), 0, st, a);
+}
+
+cudaError_t launch_pages_fork(const llx_pages_args& a, cudaStream_t st) {
+  if (a.n == 0) return cudaSuccess;
+  const cudaError_t e = launch_k(k_pages_fork, dim3(1), dim3(kPlanThreads), 0, st, a);
+  if (e != cudaSuccess) return e;
+  return launch_k(k_pages_fork_copy, dim3(copy_grid(a.n * a.max_pages * a.n_layers * 2)), dim3(256), 0, st, a);
+}
+
+cudaError_t launch_pages_compact(const llx_pages_args& a, cudaStream_t st) {
+  const cudaError_t e = launch_k(k_pages_compact, dim3(1), dim3(kPlanThreads), 0, st, a);
+  if (e != cudaSuccess) return e;
+  return launch_k(k_pages_compact_move, dim3(copy_grid(a.n_pages * a.n_layers * 2)), dim3(256), 0, st, a);
+}
+
+}  // namespace llx

@@ -1,0 +1,165 @@
+// Causal GQA integer-softmax attention of a ragged launch over a paged int8 cache
+// (numerics.h:88-120, golden.py:353-366): every row's maximum over all its keys, then the sum of
+// the table exponentials, then the normalised integer weights times the values.  Max and sums are
+// integer, so any split of the keys gives the reference's bits.
+#include <cuda_runtime.h>
+
+#include <climits>
+#include <cstdint>
+
+#include "device_luts.h"
+#include "launch.cuh"
+#include "numerics.cuh"
+#include "paged.h"
+
+namespace llx {
+
+// One sequence of a launch as the kernels see it.
+struct SeqView {
+  int slot;
+  int rows;     // rows of the launch, at most max_rows
+  int first;    // launch row of its first one
+  int64_t len;  // positions it has, clamped to what the table and the call's bound hold
+  int code;
+};
+
+__device__ __forceinline__ SeqView view_sequence(const llx_paged_attention_args& a, int i) {
+  SeqView v;
+  v.code = 0;
+  v.first = a.q_start[i];
+  const int end = a.q_start[i + 1];
+  v.rows = end - v.first;
+  v.slot = a.seqs ? a.seqs[i] : i;
+  v.len = 0;
+  if (v.rows < 0 || v.first < 0 || end > a.rows) {
+    v.rows = 0;
+    v.code = LLX_STATUS_BAD_BOUND;
+    return v;
+  }
+  if (v.slot < 0 || v.slot >= a.max_seqs) {
+    v.code = LLX_STATUS_BAD_SLOT;
+    v.slot = -1;
+    return v;
+  }
+  v.len = a.length[v.slot];
+  return v;
+}
+
+template <typename T, typename Op>
+__device__ __forceinline__ T reduce_block(T v, T* scratch, Op op) {
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, nw = blockDim.x >> 5;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
+  __syncthreads();
+  if (lane == 0) scratch[w] = v;
+  __syncthreads();
+  T r = scratch[0];
+  for (int i = 1; i < nw; ++i) r = op(r, scratch[i]);
+  return r;
+}
+
+// Any geometry: one block per (row, query head), three passes over the keys, scores recomputed.
+__global__ void __launch_bounds__(256) k_paged_attention_any(const llx_paged_attention_args a) {
+  pdl_trigger();
+  pdl_wait();
+  __shared__ __align__(16) int8_t q_s[256];
+  __shared__ int32_t pn_s[256];
+  __shared__ int32_t acc_s[256];
+  __shared__ long long red[8];
+  __shared__ uint16_t expi[16], expf[256];
+  const int r = blockIdx.x, h = blockIdx.y;
+  const int D = (int)a.head_dim, rep = (int)(a.n_heads / a.n_kv_heads), kvh = h / rep;
+  const int i = find_sequence(a.q_start, (int)a.n_seqs, r);
+  if (i < 0) return;
+  const SeqView sv = view_sequence(a, i);
+  const int64_t P = a.page_size;
+  int code = sv.code;
+  // keys 0 .. T - 1; the bounds of the call and of the page table cut both
+  int64_t T = sv.slot < 0 ? 0 : sv.len - sv.rows + (r - sv.first) + 1;
+  if (T <= 0 && !code) code = LLX_STATUS_BAD_POSITION;
+  if (r - sv.first >= a.max_rows) {
+    if (threadIdx.x == 0) raise_status(a.status, LLX_STATUS_BAD_BOUND);
+    return;
+  }
+  const int64_t cap = min(a.max_len, a.max_pages * P);
+  if (T > cap) {
+    code |= LLX_STATUS_BAD_BOUND;
+    T = cap;
+  }
+  for (int e = threadIdx.x; e < D; e += blockDim.x) q_s[e] = a.q8[r * a.q8_stride + h * D + e];
+  expf[threadIdx.x] = kDevExpF[threadIdx.x];
+  if (threadIdx.x < 16) expi[threadIdx.x] = kDevExpI[threadIdx.x];
+  acc_s[threadIdx.x] = 0;
+  __syncthreads();
+  const int32_t* pages = a.table + (sv.slot < 0 ? 0 : sv.slot) * a.table_stride;
+  bool bad = false;
+  auto page_of = [&](int64_t t) {
+    const int id = pages[t / P];
+    return id < 0 || id >= a.n_pages ? (int64_t)-1 : id * a.page_stride + (kvh * P + t % P) * D;
+  };
+  auto score = [&](int64_t at) {
+    const uint4* k = reinterpret_cast<const uint4*>(a.k_pages + at);
+    int s = 0;
+    for (int c = 0; c < D / 16; ++c) {
+      const uint4 x = k[c], y = reinterpret_cast<const uint4*>(q_s)[c];
+      s = __dp4a((int)x.x, (int)y.x, s);
+      s = __dp4a((int)x.y, (int)y.y, s);
+      s = __dp4a((int)x.z, (int)y.z, s);
+      s = __dp4a((int)x.w, (int)y.w, s);
+    }
+    return s;
+  };
+  long long mx = LLONG_MIN;
+  for (int64_t t = threadIdx.x; t < T; t += blockDim.x) {
+    const int64_t at = page_of(t);
+    if (at < 0)
+      bad = true;
+    else
+      mx = max(mx, (long long)score(at));
+  }
+  if (bad) code |= LLX_STATUS_BAD_PAGE;
+  if (code) raise_status(a.status, code);
+  mx = reduce_block<long long>(mx, red, [](long long x, long long y) { return x > y ? x : y; });
+  long long sum = 0;
+  for (int64_t t = threadIdx.x; t < T; t += blockDim.x) {
+    const int64_t at = page_of(t);
+    if (at >= 0) sum += exp_prob(mulshift(mx - score(at), a.Ms, (int)a.Ss), expi, expf);
+  }
+  sum = reduce_block<long long>(sum, red, [](long long x, long long y) { return x + y; });
+  const int64_t inv = (int64_t)(((uint64_t)1 << 31) / (uint64_t)(sum ? sum : 1));
+  const int64_t pmax = (1 << a.prob_bits) - 1;
+  const int groups = 256 / D, d = threadIdx.x % D, g = threadIdx.x / D;
+  int32_t acc = 0;
+  for (int64_t t0 = 0; t0 < T; t0 += 256) {
+    const int64_t t = t0 + threadIdx.x;
+    int32_t pn = 0;
+    if (t < T) {
+      const int64_t at = page_of(t);
+      if (at >= 0) {
+        const int64_t p = exp_prob(mulshift(mx - score(at), a.Ms, (int)a.Ss), expi, expf);
+        pn = (int32_t)min(rshr(p * inv, 31 - (int)a.prob_bits), pmax);
+      }
+    }
+    __syncthreads();
+    pn_s[threadIdx.x] = pn;
+    __syncthreads();
+    if (g < groups)
+      for (int x = g; x < 256 && t0 + x < T; x += groups)
+        if (pn_s[x]) acc += pn_s[x] * a.v_pages[page_of(t0 + x) + d];  // pn > 0: its page is there
+  }
+  __syncthreads();
+  if (g < groups) atomicAdd(&acc_s[d], acc);  // integer: any order
+  __syncthreads();
+  for (int e = threadIdx.x; e < D; e += blockDim.x) {
+    int64_t o = acc_s[e];
+    if (a.prob_bits == 15) o = rshr(o, 7);
+    a.out[r * a.out_stride + h * D + e] = (int8_t)sat8(mulshift(o, a.Mo, (int)a.So));
+  }
+}
+
+cudaError_t launch_paged_attention(const llx_paged_attention_args& a, cudaStream_t st) {
+  if (a.rows == 0 || a.n_seqs == 0) return cudaSuccess;
+  return launch_k(k_paged_attention_any, dim3((unsigned)a.rows, (unsigned)a.n_heads), dim3(256), 0, st, a);
+}
+
+}  // namespace llx

@@ -61,6 +61,15 @@ SIGNATURES = {
     "llx_binary_version": (C.c_int, [C.c_int, C.c_void_p]),
     "llx_tp_unique_id": (C.c_int, [C.c_void_p]),
     "llx_tp_init": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int]),
+    # the paged-serving calls take their argument struct as packed bytes (paged.py, sampling.py)
+    "llx_paged_append": (C.c_int, [C.c_char_p, C.c_void_p]),
+    "llx_paged_attention": (C.c_int, [C.c_char_p, C.c_void_p]),
+    "llx_pages_scratch": (C.c_size_t, [C.c_int64]),
+    "llx_pages_reserve": (C.c_int, [C.c_char_p, C.c_void_p]),
+    "llx_pages_fork": (C.c_int, [C.c_char_p, C.c_void_p]),
+    "llx_pages_free": (C.c_int, [C.c_char_p, C.c_void_p]),
+    "llx_pages_compact": (C.c_int, [C.c_char_p, C.c_void_p]),
+    "llx_sample": (C.c_int, [C.c_char_p, C.c_void_p]),
 }
 
 
