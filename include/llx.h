@@ -196,6 +196,7 @@ llx_status llx_linear_argmax_noalloc(const int8_t* A, const int8_t* W, const int
 #define LLX_STATUS_NO_PAGES 8      /* too few free pages: nothing was changed */
 #define LLX_STATUS_BAD_SLOT 16     /* a slot outside the table, listed twice, or both parent and child */
 #define LLX_STATUS_SHARED_PAGE 32  /* new positions would fall into a page that others share */
+#define LLX_STATUS_LOST 64         /* a bounded wait of a kernel ran out: the call's results are void */
 
 /* q [rows][n_heads][head_dim], k [rows][n_kv_heads][head_dim] i16 and v (i8) of the launch: norm
  * of every query and key head (gamma null: none), rotation (cos / sin [n_positions][head_dim / 2]

@@ -4,46 +4,9 @@
 // integer, so any split of the keys gives the reference's bits.
 #include <cuda_runtime.h>
 
-#include <climits>
-#include <cstdint>
-
-#include "device_luts.h"
-#include "launch.cuh"
-#include "numerics.cuh"
-#include "paged.h"
+#include "paged_attn.cuh"
 
 namespace llx {
-
-// One sequence of a launch as the kernels see it.
-struct SeqView {
-  int slot;
-  int rows;     // rows of the launch, at most max_rows
-  int first;    // launch row of its first one
-  int64_t len;  // positions it has, clamped to what the table and the call's bound hold
-  int code;
-};
-
-__device__ __forceinline__ SeqView view_sequence(const llx_paged_attention_args& a, int i) {
-  SeqView v;
-  v.code = 0;
-  v.first = a.q_start[i];
-  const int end = a.q_start[i + 1];
-  v.rows = end - v.first;
-  v.slot = a.seqs ? a.seqs[i] : i;
-  v.len = 0;
-  if (v.rows < 0 || v.first < 0 || end > a.rows) {
-    v.rows = 0;
-    v.code = LLX_STATUS_BAD_BOUND;
-    return v;
-  }
-  if (v.slot < 0 || v.slot >= a.max_seqs) {
-    v.code = LLX_STATUS_BAD_SLOT;
-    v.slot = -1;
-    return v;
-  }
-  v.len = a.length[v.slot];
-  return v;
-}
 
 template <typename T, typename Op>
 __device__ __forceinline__ T reduce_block(T v, T* scratch, Op op) {
@@ -157,8 +120,35 @@ __global__ void __launch_bounds__(256) k_paged_attention_any(const llx_paged_att
   }
 }
 
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+cudaError_t make_page_map(CUtensorMap* map, const void* base, const llx_paged_attention_args& a, int box_rows) {
+  static const EncodeTiled encode = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      f = nullptr;
+    return reinterpret_cast<EncodeTiled>(f);
+  }();
+  if (!encode) return cudaErrorNotSupported;
+  const cuuint64_t dims[3] = {(cuuint64_t)a.head_dim, (cuuint64_t)(a.n_kv_heads * a.page_size), (cuuint64_t)a.n_pages};
+  const cuuint64_t strides[2] = {(cuuint64_t)a.head_dim, (cuuint64_t)a.page_stride};
+  const cuuint32_t box[3] = {(cuuint32_t)a.head_dim, (cuuint32_t)box_rows, 1};
+  const cuuint32_t step[3] = {1, 1, 1};
+  const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, step,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            a.head_dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
 cudaError_t launch_paged_attention(const llx_paged_attention_args& a, cudaStream_t st) {
-  if (a.rows == 0 || a.n_seqs == 0) return cudaSuccess;
+  if (a.rows == 0 || a.n_seqs == 0 || a.max_rows == 0) return cudaSuccess;
+  const int64_t pairs = a.max_rows * (a.n_heads / a.n_kv_heads);
+  if (pairs <= 32 && paged_decode_fits(a, pairs)) return launch_paged_decode(a, 32, st);
   return launch_k(k_paged_attention_any, dim3((unsigned)a.rows, (unsigned)a.n_heads), dim3(256), 0, st, a);
 }
 

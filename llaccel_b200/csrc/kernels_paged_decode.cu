@@ -1,0 +1,420 @@
+// Paged attention of few query rows per sequence (decode steps, a handful of draft tokens).
+//
+// A cluster of C CTAs serves one (sequence, KV head, group of up to 8 stacked (row, head) pairs);
+// each CTA takes a slice of the keys.  One thread streams the slice's K rows, then its V rows,
+// page by page through a ring of TMA-filled stages; four warps consume them, so every byte of the
+// cache is read once:
+//   scores  S^T (16 keys x 8 pairs) = K (16 x 32) Q^T per int8 MMA, kept in shared memory;
+//   maxima  of the slices meet in every CTA of the cluster (the reference's global maximum);
+//   table exponentials in place, and their sums meet the same way;
+//   values  O^T (16 channels x 8 pairs) += V^T (16 x 32 keys) P^T with the weights normalised on
+//           the way into the MMA as two unsigned bytes, O = 256 hi + lo;
+//   partial outputs are added by the CTA that finishes them, 1/C of the outputs each.
+// Integer maxima and sums: any split gives the same bits.
+#include <atomic>
+
+#include "paged_attn.cuh"
+
+namespace llx {
+namespace {
+
+constexpr int kConsumers = 128, kThreads = 160;  // four warps and the loading warp
+constexpr int kPairs = 8;                        // stacked (row, head) pairs per CTA
+constexpr int kTK = 128;                         // keys per stage: 32 per warp
+constexpr int kMaxCluster = 16;
+template <int D>
+constexpr int kRing = D == 128 ? 3 : 4;  // 48 KB / 32 KB in flight per CTA
+
+// row stride of the scores in words, = 8 mod 32: a warp's 8-byte reads of 4 pairs x 8 keys and its
+// stores hit different banks
+__host__ __device__ constexpr int score_stride(int cap) { return (cap + 31) / 32 * 32 + 8; }
+
+struct DecodeShape {
+  int cluster, cap, box;  // CTAs per cluster, keys per slice (multiple of 64), rows per TMA box
+  int nr;                 // score rows held
+};
+
+template <int D>
+__host__ __device__ inline size_t decode_smem(int nr, int cap, int P) {
+  return 1024 + (size_t)kRing<D> * kTK * D + (size_t)nr * score_stride(cap) * 4 + (size_t)2 * nr * D * 4 +
+         (size_t)(cap / P + 2) * 4;
+}
+
+template <int D, bool HIGH>
+__global__ void __launch_bounds__(kThreads) k_paged_decode(const llx_paged_attention_args a, const __grid_constant__ CUtensorMap mk,
+                                                           const __grid_constant__ CUtensorMap mv, const DecodeShape shape,
+                                                           const int most) {
+  constexpr int S = kRing<D>, KB = D / 32, MB = D / 16;
+  extern __shared__ unsigned char raw[];
+  __shared__ __align__(8) uint64_t full[S], empty[S], met[3];
+  __shared__ int lost, any_bad;
+  __shared__ uint32_t xmax[kMaxCluster * kPairs], xsum[kMaxCluster * kPairs], wred[4 * kPairs];
+  __shared__ uint16_t expi[18], expf[256];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int C = shape.cluster;
+  const uint32_t rank = C > 1 ? pa::cluster_rank() : 0;
+  if (tid == 0) {
+    for (int s = 0; s < S; ++s) {
+      pa::bar_init(&full[s], 1);
+      pa::bar_init(&empty[s], kConsumers / 32);
+    }
+    for (int s = 0; s < 3; ++s) pa::bar_init(&met[s], C);
+    lost = any_bad = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  for (int x = tid; x < 256; x += kThreads) expf[x] = kDevExpF[x];
+  if (tid < 18) expi[tid] = tid < 16 ? kDevExpI[tid] : 0;
+  pdl_trigger();
+  pdl_wait();
+  const int i = blockIdx.x / C, kvh = blockIdx.y;
+  const SeqView sv = view_sequence(a, i);
+  const int rep = (int)(a.n_heads / a.n_kv_heads), P = (int)a.page_size;
+  const int rows = min(sv.rows, (int)min(a.max_rows, (int64_t)INT_MAX));
+  const int64_t pairs = (int64_t)rows * rep;
+  const int g0 = blockIdx.z * kPairs;
+  if (pairs > most || g0 >= pairs) {  // the whole cluster agrees
+    if (sv.code && rank == 0 && kvh == 0 && g0 == 0 && tid == 0) raise_status(a.status, sv.code);
+    return;
+  }
+  const int nr = min(kPairs, (int)pairs - g0);
+  // row j of the sequence sees keys 0 .. len - rows + j
+  const int cap = key_cap(a);
+  auto keys_of = [&](int n) {  // of pair g0 + n
+    const int64_t t = (int64_t)sv.len - sv.rows + (g0 + n) / rep + 1;
+    return (int)(t < 0 ? 0 : t > cap ? cap : t);
+  };
+  const int T = keys_of(nr - 1);
+  int slice = ((T + C - 1) / C + 63) & ~63;
+  const int k0 = (int)min((int64_t)T, (int64_t)rank * slice), k1 = (int)min((int64_t)T, (int64_t)k0 + slice), nkeys = k1 - k0;
+  const int tiles = (nkeys + kTK - 1) / kTK;
+  const int ss = score_stride(shape.cap);
+  unsigned char* base = raw + ((1024 - (pa::s32(raw) & 1023)) & 1023);
+  unsigned char* ring = base;
+  int32_t* sc = reinterpret_cast<int32_t*>(base + S * kTK * D);  // [nr][ss]
+  int32_t* opart = sc + shape.nr * ss;                            // [nr][D] this slice's sums
+  int32_t* xo = opart + shape.nr * D;                             // [C][nr * D / C] peers' sums of this CTA's share
+  int32_t* ids = xo + shape.nr * D;                               // page ids of the slice
+  const int p0 = k0 / P, np = nkeys ? (k1 - 1) / P - p0 + 1 : 0;
+  const int32_t* pages = a.table + (sv.slot < 0 ? 0 : sv.slot) * a.table_stride + p0;
+  __syncthreads();
+  for (int x = tid; x < np; x += kThreads) {
+    int id = pages[x];
+    if (id < 0 || id >= a.n_pages) {
+      id = -1;
+      any_bad = 1;
+    }
+    ids[x] = id;
+  }
+  for (int x = tid; x < nr * D; x += kThreads) opart[x] = 0;
+  if (C > 1)
+    pa::cluster_sync();  // the peers' barriers are there
+  else
+    __syncthreads();
+  if (rank == 0 && kvh == 0 && tid == 0) {
+    int code = sv.code;
+    if (sv.rows > a.max_rows || sv.len > cap) code |= LLX_STATUS_BAD_BOUND;
+    if (!code && sv.len < sv.rows) code = LLX_STATUS_BAD_POSITION;
+    if (code) raise_status(a.status, code);
+  }
+  if (tid == 0 && any_bad) raise_status(a.status, LLX_STATUS_BAD_PAGE);
+
+  if (warp == kConsumers / 32) {
+    if (lane == 0) {
+      for (int it = 0; it < 2 * tiles; ++it) {
+        const int s = it % S, t0 = (it < tiles ? it : it - tiles) * kTK;
+        if (it >= S && !pa::bar_wait(&empty[s], (uint32_t)(it / S - 1) & 1, &lost)) break;
+        const int boxes = (min(kTK, nkeys - t0) + shape.box - 1) / shape.box;
+        pa::bar_expect(&full[s], (uint32_t)(boxes * shape.box * D));
+        for (int b = 0; b < boxes; ++b) {
+          const int key = k0 + t0 + b * shape.box;
+          // absent pages: page 0 is read in their place, its keys are never used
+          pa::load_rows(ring + s * kTK * D + b * shape.box * D, it < tiles ? &mk : &mv, &full[s], kvh * P + key % P,
+                        max(ids[key / P - p0], 0));
+        }
+      }
+    }
+  } else {
+    const int g = lane >> 2, tig = lane & 3;
+    // ---- scores ----
+    uint32_t qf[KB][2];
+    {
+      const int n = g0 + g;
+      const int8_t* q = a.q8 + (int64_t)(sv.first + n / rep) * a.q8_stride + (int64_t)(kvh * rep + n % rep) * D + 4 * tig;
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        qf[kb][0] = g < nr ? *reinterpret_cast<const uint32_t*>(q + kb * 32) : 0u;
+        qf[kb][1] = g < nr ? *reinterpret_cast<const uint32_t*>(q + kb * 32 + 16) : 0u;
+      }
+    }
+    const int ra = 2 * tig, rb = ra + 1;
+    const int Ta = ra < nr ? keys_of(ra) - k0 : 0, Tb = rb < nr ? keys_of(rb) - k0 : 0;  // visible keys of the slice
+    int mxa = INT_MIN, mxb = INT_MIN;
+    for (int it = 0; it < tiles; ++it) {
+      const int s = it % S;
+      pa::bar_wait(&full[s], (uint32_t)(it / S) & 1, &lost);
+      const int t0 = it * kTK + warp * 32;
+      if (t0 < nkeys) {
+        const uint32_t tile = pa::s32(ring + s * kTK * D);
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          int32_t c[4] = {0, 0, 0, 0};
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb) {
+            uint32_t f[4];
+            pa::ldmatrix4(f, tile + pa::tile_at<D>(warp * 32 + m * 16 + (lane & 15), kb * 2 + (lane >> 4)));
+            pa::mma16832<false>(c, f[0], f[1], f[2], f[3], qf[kb][0], qf[kb][1]);
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int t = t0 + m * 16 + h * 8 + g;  // key of the slice
+            const bool there = !any_bad || t >= nkeys || ids[(k0 + t) / P - p0] >= 0;
+            const int va = t < Ta && there ? c[2 * h] : INT_MIN, vb = t < Tb && there ? c[2 * h + 1] : INT_MIN;
+            if (ra < nr) sc[ra * ss + t] = va;
+            if (rb < nr) sc[rb * ss + t] = vb;
+            mxa = max(mxa, va);
+            mxb = max(mxb, vb);
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) pa::bar_arrive(&empty[s]);
+    }
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) {
+      mxa = max(mxa, __shfl_xor_sync(0xffffffffu, mxa, o));
+      mxb = max(mxb, __shfl_xor_sync(0xffffffffu, mxb, o));
+    }
+    if (g == 0) {
+      wred[warp * kPairs + ra] = (uint32_t)mxa;
+      wred[warp * kPairs + rb] = (uint32_t)mxb;
+    }
+    pa::named_sync(1, kConsumers);
+    // every CTA of the cluster gets every slice's maxima: x[slice][pair]
+    auto meet = [&](uint32_t v, uint32_t* x, uint64_t* bar) {  // thread c * kPairs + n brings pair n to CTA c
+      const int n = tid % kPairs, c = tid / kPairs;
+      if (C == 1) {
+        if (tid < kPairs) x[n] = v;
+        pa::named_sync(1, kConsumers);
+        return;
+      }
+      if (c < C) pa::peer_store(pa::peer(x + rank * kPairs + n, (uint32_t)c), v);
+      pa::named_sync(1, kConsumers);
+      if (tid < C) pa::peer_arrive(pa::peer(bar, (uint32_t)tid));
+      pa::bar_wait_cluster(bar, 0, &lost);
+    };
+    {
+      int v = INT_MIN;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) v = max(v, (int)wred[w * kPairs + tid % kPairs]);
+      meet((uint32_t)v, xmax, &met[0]);
+    }
+    // ---- exponentials of the slice, in place; sums ----
+    const int nfill = (nkeys + 31) & ~31;  // the score pass wrote up to here
+    const GapScale gs = gap_scale(a.Ms, a.Ss);
+    {
+      int mx[kPairs];
+      uint32_t sum[kPairs];
+#pragma unroll
+      for (int n = 0; n < kPairs; ++n) {
+        mx[n] = INT_MIN;
+        sum[n] = 0;
+        for (int c = 0; c < C; ++c) mx[n] = max(mx[n], (int)xmax[c * kPairs + n]);
+      }
+      for (int t = tid; t < nfill; t += kConsumers) {
+#pragma unroll
+        for (int n = 0; n < kPairs; ++n) {
+          if (n < nr) {
+            const int v = sc[n * ss + t];
+            const uint32_t e = table_exp(gap_index<HIGH>((uint32_t)mx[n] - (uint32_t)v, gs), expi, expf);
+            const uint32_t p = v == INT_MIN ? 0u : e;
+            sc[n * ss + t] = (int)p;
+            sum[n] += p;
+          }
+        }
+      }
+      // a slice has less than 2^16 keys of at most 65535: 32 bits hold its sum
+      pa::named_sync(1, kConsumers);  // wred is free again
+#pragma unroll
+      for (int n = 0; n < kPairs; ++n) {
+        const uint32_t v = __reduce_add_sync(0xffffffffu, sum[n]);
+        if (lane == n) wred[warp * kPairs + n] = v;
+      }
+      pa::named_sync(1, kConsumers);
+    }
+    {
+      uint32_t v = 0;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) v += wred[w * kPairs + tid % kPairs];
+      meet(v, xsum, &met[1]);
+    }
+    // ---- values: weights of pair g, normalised as they are read ----
+    uint64_t whole = 0;
+    for (int c = 0; c < C; ++c) whole += xsum[c * kPairs + g];
+    const uint32_t inv = whole > 0x80000000ull ? 0u : 0x80000000u / (whole ? (uint32_t)whole : 1u);
+    const int psh = 31 - (int)a.prob_bits;
+    const uint32_t prnd = 1u << (psh - 1), pmax = (1u << a.prob_bits) - 1u;
+    const bool wide = a.prob_bits > 8;
+    int32_t ah[MB][4], al[MB][4];
+#pragma unroll
+    for (int m = 0; m < MB; ++m)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) ah[m][k] = al[m][k] = 0;
+    for (int it = tiles; it < 2 * tiles; ++it) {
+      const int s = it % S;
+      pa::bar_wait(&full[s], (uint32_t)(it / S) & 1, &lost);
+      const int t0 = (it - tiles) * kTK + warp * 32;
+      if (t0 < nkeys) {
+        const unsigned char* tile = ring + s * kTK * D;
+        // MMA key index 4 tig + e of a 16-key half stands for key 2 tig + (e & 1) + 8 (e >> 1),
+        // in the weights as in the values: the 16-byte reads of a quarter warp then hit 8 chunks
+        uint32_t w[2][MB * 2], bl[2], bh[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t pn[4] = {0, 0, 0, 0};
+          if (g < nr) {
+            const int2 x = *reinterpret_cast<const int2*>(sc + g * ss + t0 + h * 16 + 2 * tig);
+            const int2 y = *reinterpret_cast<const int2*>(sc + g * ss + t0 + h * 16 + 2 * tig + 8);
+            // p <= sum, so p * inv <= 2^31
+            pn[0] = min(((uint32_t)x.x * inv + prnd) >> psh, pmax);
+            pn[1] = min(((uint32_t)x.y * inv + prnd) >> psh, pmax);
+            pn[2] = min(((uint32_t)y.x * inv + prnd) >> psh, pmax);
+            pn[3] = min(((uint32_t)y.y * inv + prnd) >> psh, pmax);
+          }
+          const uint32_t p01 = __byte_perm(pn[0], pn[1], 0x5410), p23 = __byte_perm(pn[2], pn[3], 0x5410);
+          bl[h] = __byte_perm(p01, p23, 0x6420);
+          bh[h] = __byte_perm(p01, p23, 0x7531);
+          const int r0 = warp * 32 + h * 16 + 2 * tig;
+          if constexpr (D == 128) {
+            uint4 v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              v[e] = *reinterpret_cast<const uint4*>(tile + pa::tile_at<D>(r0 + (e & 1) + 8 * (e >> 1), g));
+            pa::transpose4(v[0].x, v[1].x, v[2].x, v[3].x, w[h]);
+            pa::transpose4(v[0].y, v[1].y, v[2].y, v[3].y, w[h] + 4);
+            pa::transpose4(v[0].z, v[1].z, v[2].z, v[3].z, w[h] + 8);
+            pa::transpose4(v[0].w, v[1].w, v[2].w, v[3].w, w[h] + 12);
+          } else {
+            uint2 v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              v[e] = *reinterpret_cast<const uint2*>(tile + pa::tile_at<D>(r0 + (e & 1) + 8 * (e >> 1), g >> 1) + (g & 1) * 8);
+            pa::transpose4(v[0].x, v[1].x, v[2].x, v[3].x, w[h]);
+            pa::transpose4(v[0].y, v[1].y, v[2].y, v[3].y, w[h] + 4);
+          }
+        }
+#pragma unroll
+        for (int m = 0; m < MB; ++m) {
+          pa::mma16832<true>(al[m], w[0][2 * m], w[0][2 * m + 1], w[1][2 * m], w[1][2 * m + 1], bl[0], bl[1]);
+          if (wide) pa::mma16832<true>(ah[m], w[0][2 * m], w[0][2 * m + 1], w[1][2 * m], w[1][2 * m + 1], bh[0], bh[1]);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) pa::bar_arrive(&empty[s]);
+    }
+    // block row g of m stands for channel g D / 8 + 2 m, row g + 8 for the next one
+#pragma unroll
+    for (int m = 0; m < MB; ++m)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int n = 2 * tig + (k & 1), ch = g * (D / 8) + 2 * m + (k >> 1);
+        if (n < nr) atomicAdd(&opart[n * D + ch], ah[m][k] * 256 + al[m][k]);
+      }
+    pa::named_sync(1, kConsumers);
+    // ---- each CTA finishes 1/C of the outputs (C divides D) ----
+    const int share = nr * D / C, e0 = (int)rank * share;
+    if (C > 1) {
+      for (int e = tid; e < nr * D; e += kConsumers) {
+        const int c = e / share;
+        pa::peer_store(pa::peer(xo + rank * share + (e - c * share), (uint32_t)c), (uint32_t)opart[e]);
+      }
+      pa::named_sync(1, kConsumers);
+      if (tid < C) pa::peer_arrive(pa::peer(&met[2], (uint32_t)tid));
+      pa::bar_wait_cluster(&met[2], 0, &lost);
+    }
+    for (int x = tid; x < share; x += kConsumers) {
+      int64_t o = 0;
+      if (C > 1)
+        for (int c = 0; c < C; ++c) o += xo[c * share + x];
+      else
+        o = opart[x];
+      if (a.prob_bits == 15) o = rshr(o, 7);
+      const int e = e0 + x, n = g0 + e / D;
+      a.out[(int64_t)(sv.first + n / rep) * a.out_stride + (int64_t)(kvh * rep + n % rep) * D + e % D] =
+          (int8_t)sat8(mulshift(o, a.Mo, (int)a.So));
+    }
+    if (lost && tid == 0) raise_status(a.status, LLX_STATUS_LOST);
+  }
+  // no CTA leaves while a peer may still write to it
+  if (C > 1) {
+    __syncwarp();
+    pa::cluster_sync();
+  }
+}
+
+template <int D, bool HIGH>
+cudaError_t launch_decode_t(const llx_paged_attention_args& a, int most, const DecodeShape& sh, int groups, cudaStream_t st) {
+  static std::atomic<bool> ready[64];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  if (!ready[dev].load(std::memory_order_acquire)) {
+    e = cudaFuncSetAttribute(k_paged_decode<D, HIGH>, cudaFuncAttributeMaxDynamicSharedMemorySize, 224 * 1024);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_paged_decode<D, HIGH>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return e;
+    ready[dev].store(true, std::memory_order_release);
+  }
+  CUtensorMap mk, mv;
+  e = make_page_map(&mk, a.k_pages, a, sh.box);
+  if (e == cudaSuccess) e = make_page_map(&mv, a.v_pages, a, sh.box);
+  if (e != cudaSuccess) return e;
+  const size_t smem = decode_smem<D>(sh.nr, sh.cap, (int)a.page_size);
+  const dim3 grid((unsigned)(a.n_seqs * sh.cluster), (unsigned)a.n_kv_heads, (unsigned)groups);
+  if (sh.cluster == 1) return launch_k(k_paged_decode<D, HIGH>, grid, dim3(kThreads), smem, st, a, mk, mv, sh, most);
+  return launch_kc(k_paged_decode<D, HIGH>, grid, dim3(kThreads), smem, st, dim3(sh.cluster, 1, 1), a, mk, mv, sh, most);
+}
+
+int slice_cap(int64_t max_len, int C) { return (int)(((max_len + C - 1) / C + 63) / 64 * 64); }
+
+size_t smem_for(const llx_paged_attention_args& a, int nr, int64_t len, int C) {
+  const int cap = slice_cap(len, C), P = (int)a.page_size;
+  return a.head_dim == 128 ? decode_smem<128>(nr, cap, P) : decode_smem<64>(nr, cap, P);
+}
+
+constexpr size_t kSmemMost = 220 * 1024;
+
+int64_t longest(const llx_paged_attention_args& a) {
+  const int64_t held = a.max_pages * a.page_size;
+  const int64_t n = a.max_len < held ? a.max_len : held;
+  return n < 1 ? 1 : n;
+}
+
+}  // namespace
+
+bool paged_decode_fits(const llx_paged_attention_args& a, int64_t pairs) {
+  if (a.head_dim != 64 && a.head_dim != 128) return false;
+  if (longest(a) > (1 << 19)) return false;  // a slice's keys and sums stay in range
+  return smem_for(a, (int)(pairs < kPairs ? pairs : kPairs), longest(a), kMaxCluster) <= kSmemMost;
+}
+
+cudaError_t launch_paged_decode(const llx_paged_attention_args& a, int most, cudaStream_t st) {
+  const int64_t rep = a.n_heads / a.n_kv_heads, len = longest(a);
+  const int64_t pairs = a.max_rows * rep < most ? a.max_rows * rep : most;
+  const int groups = (int)((pairs + kPairs - 1) / kPairs);
+  DecodeShape sh;
+  sh.nr = (int)(pairs < kPairs ? pairs : kPairs);
+  sh.box = a.page_size < 64 ? (int)a.page_size : 64;
+  const int64_t units = a.n_seqs * a.n_kv_heads * groups;
+  // Split the keys until two CTAs per SM have work, as long as a slice keeps a stage of keys; and
+  // further where the scores would not leave room for two CTAs on an SM.
+  int C = 1;
+  while (C < kMaxCluster && ((units * C < 2 * 148 && len > (int64_t)C * kTK) || smem_for(a, sh.nr, len, C) > 110 * 1024)) C *= 2;
+  while (C < kMaxCluster && smem_for(a, sh.nr, len, C) > kSmemMost) C *= 2;
+  sh.cluster = C;
+  sh.cap = slice_cap(len, C);
+  if (a.head_dim == 128)
+    return a.Ss >= 33 ? launch_decode_t<128, true>(a, most, sh, groups, st) : launch_decode_t<128, false>(a, most, sh, groups, st);
+  return a.Ss >= 33 ? launch_decode_t<64, true>(a, most, sh, groups, st) : launch_decode_t<64, false>(a, most, sh, groups, st);
+}
+
+}  // namespace llx

@@ -35,7 +35,8 @@ STATUS = {1: "a position's page id lies outside the cache",
           4: "a sequence with more rows or positions than the call was told",
           8: "too few free pages",
           16: "a slot outside the table, listed twice, or both parent and child",
-          32: "new positions would fall into a page that other sequences share"}
+          32: "new positions would fall into a page that other sequences share",
+          64: "a bounded wait of a kernel ran out: the call's results are void"}
 
 _APPEND = struct.Struct("=42q")
 _ATTENTION = struct.Struct("=30q")
