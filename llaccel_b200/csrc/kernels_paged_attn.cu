@@ -148,7 +148,15 @@ cudaError_t make_page_map(CUtensorMap* map, const void* base, const llx_paged_at
 cudaError_t launch_paged_attention(const llx_paged_attention_args& a, cudaStream_t st) {
   if (a.rows == 0 || a.n_seqs == 0 || a.max_rows == 0) return cudaSuccess;
   const int64_t pairs = a.max_rows * (a.n_heads / a.n_kv_heads);
-  if (pairs <= 32 && paged_decode_fits(a, pairs)) return launch_paged_decode(a, 32, st);
+  constexpr int kFew = 32;
+  if (paged_chunk_fits(a)) {
+    if (!paged_decode_fits(a, pairs < kFew ? pairs : kFew)) return launch_paged_chunk(a, 0, st);
+    if (pairs <= kFew) return launch_paged_decode(a, kFew, st);
+    // sequences of both kinds, unless all have the most rows
+    if (a.n_seqs * a.max_rows == a.rows) return launch_paged_chunk(a, 0, st);
+    const cudaError_t e = launch_paged_chunk(a, kFew + 1, st);
+    return e != cudaSuccess ? e : launch_paged_decode(a, kFew, st);
+  }
   return launch_k(k_paged_attention_any, dim3((unsigned)a.rows, (unsigned)a.n_heads), dim3(256), 0, st, a);
 }
 

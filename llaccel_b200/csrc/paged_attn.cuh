@@ -210,4 +210,8 @@ cudaError_t make_page_map(CUtensorMap* map, const void* base, const llx_paged_at
 bool paged_decode_fits(const llx_paged_attention_args& a, int64_t pairs);
 cudaError_t launch_paged_decode(const llx_paged_attention_args& a, int most, cudaStream_t st);
 
+// Sequences with at least `least` stacked (row, head) pairs per KV head, any length.
+bool paged_chunk_fits(const llx_paged_attention_args& a);
+cudaError_t launch_paged_chunk(const llx_paged_attention_args& a, int64_t least, cudaStream_t st);
+
 }  // namespace llx
