@@ -38,13 +38,19 @@ def pow2_table():
     return [round(2.0 ** 31 * 2.0 ** (-j / 1024.0)) for j in range(1024)]
 
 
+def curve_table():
+    """The table exponential of every index z below 4096 (NUMERICS.md:160-161)."""
+    _, expi, expf = tables()
+    return [(expi[z >> 8] * expf[z & 255] + 32768) >> 16 for z in range(4096)]
+
+
 def render_device() -> str:
     _, expi, expf = tables()
     out = ["// Generated by gen_luts.py -- integer tables in device memory.", "#pragma once", "#include <cstdint>", "",
            "namespace llx {"]
     for ctype, name, vals in (("uint16_t", "kDevExpI", expi), ("uint16_t", "kDevExpF", expf),
-                              ("uint32_t", "kDevPow2", pow2_table())):
-        out.append(f"static __device__ const {ctype} {name}[{len(vals)}] = {{")
+                              ("uint32_t", "kDevCurve", curve_table()), ("uint32_t", "kDevPow2", pow2_table())):
+        out.append(f"static __device__ const __align__(16) {ctype} {name}[{len(vals)}] = {{")
         for i in range(0, len(vals), 8):
             out.append("    " + ", ".join(f"{v}u" for v in vals[i : i + 8]) + ",")
         out.append("};")

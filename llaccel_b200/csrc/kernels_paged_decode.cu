@@ -69,6 +69,7 @@ __global__ void __launch_bounds__(kThreads) k_paged_decode(const llx_paged_atten
   const int i = blockIdx.x / C, kvh = blockIdx.y;
   const SeqView sv = view_sequence(a, i);
   const int rep = (int)(a.n_heads / a.n_kv_heads), P = (int)a.page_size;
+  const int pshift = 31 - __clz(P);  // pages hold a power of two
   const int rows = min(sv.rows, (int)min(a.max_rows, (int64_t)INT_MAX));
   const int64_t pairs = (int64_t)rows * rep;
   const int g0 = blockIdx.z * kPairs;
@@ -94,7 +95,7 @@ __global__ void __launch_bounds__(kThreads) k_paged_decode(const llx_paged_atten
   int32_t* opart = sc + shape.nr * ss;                            // [nr][D] this slice's sums
   int32_t* xo = opart + shape.nr * D;                             // [C][nr * D / C] peers' sums of this CTA's share
   int32_t* ids = xo + shape.nr * D;                               // page ids of the slice
-  const int p0 = k0 / P, np = nkeys ? (k1 - 1) / P - p0 + 1 : 0;
+  const int p0 = k0 >> pshift, np = nkeys ? ((k1 - 1) >> pshift) - p0 + 1 : 0;
   const int32_t* pages = a.table + (sv.slot < 0 ? 0 : sv.slot) * a.table_stride + p0;
   __syncthreads();
   for (int x = tid; x < np; x += kThreads) {
@@ -120,16 +121,17 @@ __global__ void __launch_bounds__(kThreads) k_paged_decode(const llx_paged_atten
 
   if (warp == kConsumers / 32) {
     if (lane == 0) {
+      const int bshift = 31 - __clz(shape.box);
       for (int it = 0; it < 2 * tiles; ++it) {
         const int s = it % S, t0 = (it < tiles ? it : it - tiles) * kTK;
         if (it >= S && !pa::bar_wait(&empty[s], (uint32_t)(it / S - 1) & 1, &lost)) break;
-        const int boxes = (min(kTK, nkeys - t0) + shape.box - 1) / shape.box;
+        const int boxes = (min(kTK, nkeys - t0) + shape.box - 1) >> bshift;
         pa::bar_expect(&full[s], (uint32_t)(boxes * shape.box * D));
         for (int b = 0; b < boxes; ++b) {
           const int key = k0 + t0 + b * shape.box;
           // absent pages: page 0 is read in their place, its keys are never used
-          pa::load_rows(ring + s * kTK * D + b * shape.box * D, it < tiles ? &mk : &mv, &full[s], kvh * P + key % P,
-                        max(ids[key / P - p0], 0));
+          pa::load_rows(ring + s * kTK * D + b * shape.box * D, it < tiles ? &mk : &mv, &full[s], kvh * P + (key & (P - 1)),
+                        max(ids[(key >> pshift) - p0], 0));
         }
       }
     }
@@ -167,7 +169,7 @@ __global__ void __launch_bounds__(kThreads) k_paged_decode(const llx_paged_atten
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const int t = t0 + m * 16 + h * 8 + g;  // key of the slice
-            const bool there = !any_bad || t >= nkeys || ids[(k0 + t) / P - p0] >= 0;
+            const bool there = !any_bad || t >= nkeys || ids[((k0 + t) >> pshift) - p0] >= 0;
             const int va = t < Ta && there ? c[2 * h] : INT_MIN, vb = t < Tb && there ? c[2 * h + 1] : INT_MIN;
             if (ra < nr) sc[ra * ss + t] = va;
             if (rb < nr) sc[rb * ss + t] = vb;
@@ -200,7 +202,7 @@ __global__ void __launch_bounds__(kThreads) k_paged_decode(const llx_paged_atten
       if (c < C) pa::peer_store(pa::peer(x + rank * kPairs + n, (uint32_t)c), v);
       pa::named_sync(1, kConsumers);
       if (tid < C) pa::peer_arrive(pa::peer(bar, (uint32_t)tid));
-      pa::bar_wait_cluster(bar, 0, &lost);
+      pa::bar_wait<true>(bar, 0, &lost);
     };
     {
       int v = INT_MIN;
@@ -210,7 +212,7 @@ __global__ void __launch_bounds__(kThreads) k_paged_decode(const llx_paged_atten
     }
     // ---- exponentials of the slice, in place; sums ----
     const int nfill = (nkeys + 31) & ~31;  // the score pass wrote up to here
-    const GapScale gs = gap_scale(a.Ms, a.Ss);
+    const GapScale gs = gap_scale<HIGH>(a.Ms, a.Ss);
     {
       int mx[kPairs];
       uint32_t sum[kPairs];
@@ -329,7 +331,7 @@ __global__ void __launch_bounds__(kThreads) k_paged_decode(const llx_paged_atten
       }
       pa::named_sync(1, kConsumers);
       if (tid < C) pa::peer_arrive(pa::peer(&met[2], (uint32_t)tid));
-      pa::bar_wait_cluster(&met[2], 0, &lost);
+      pa::bar_wait<true>(&met[2], 0, &lost);
     }
     for (int x = tid; x < share; x += kConsumers) {
       int64_t o = 0;

@@ -57,15 +57,14 @@ __device__ __forceinline__ int key_cap(const llx_paged_attention_args& a) {
 // high word and constant to stay in 32 bits: 2^23 + 2^30 at most, for Ss <= 63.
 struct GapScale {
   uint32_t M, round;
-  int shift;  // of the high word, or of the whole product
-  bool high;
+  int shift;  // HIGH: of the high word; else of the whole product
 };
+template <bool HIGH>
 __device__ __forceinline__ GapScale gap_scale(int64_t Ms, int64_t Ss) {
   GapScale g;
   g.M = (uint32_t)Ms;
-  g.high = Ss >= 33;
-  g.shift = (int)(g.high ? Ss - 32 : Ss);
-  g.round = g.high ? 1u << (Ss - 33) : 0u;
+  g.shift = (int)(HIGH ? Ss - 32 : Ss);
+  g.round = HIGH ? 1u << (Ss - 33) : 0u;
   return g;
 }
 template <bool HIGH>
@@ -83,8 +82,9 @@ __device__ __forceinline__ uint32_t table_exp(uint32_t z, const uint16_t* expi, 
 
 namespace pa {
 
-constexpr uint32_t kPolls = 1u << 22;     // of a wait that should end
-constexpr uint32_t kPollsLost = 1u << 10;  // after one has not
+// A try suspends the thread for up to kSuspend ns instead of taking issue slots; kPolls of them
+// (over a second) bound a wait.
+constexpr uint32_t kSuspend = 20000, kPolls = 1u << 16;
 
 __device__ __forceinline__ uint32_t s32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void bar_init(uint64_t* b, uint32_t n) {
@@ -96,40 +96,46 @@ __device__ __forceinline__ void bar_arrive(uint64_t* b) {
 __device__ __forceinline__ void bar_expect(uint64_t* b, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(s32(b)), "r"(bytes) : "memory");
 }
-// Waits for a phase; false once it has not come within the limit (`lost` then stays set and
-// makes the block's later waits short, so that it ends).
-__device__ __forceinline__ bool bar_wait(uint64_t* b, uint32_t parity, volatile int* lost) {
-  const uint32_t limit = *lost ? kPollsLost : kPolls;
-  for (uint32_t i = 0; i < limit; ++i) {
-    uint32_t ok;
+template <bool CLUSTER>
+__device__ __forceinline__ bool bar_try(uint64_t* b, uint32_t parity) {
+  uint32_t ok;
+  if (CLUSTER)  // for a barrier that other CTAs of the cluster arrive on
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
         "selp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(ok)
-        : "r"(s32(b)), "r"(parity)
+        : "r"(s32(b)), "r"(parity), "r"(kSuspend)
         : "memory");
-    if (ok) return true;
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(s32(b)), "r"(parity), "r"(kSuspend)
+        : "memory");
+  return ok != 0;
+}
+// Waits for a phase; false once it has not come within the limit.  `lost` then stays set and makes
+// the block's later waits short, so that it ends.  The first try reads nothing else: a loop of
+// waits that have ended already is as fast as their tries.
+template <bool CLUSTER = false>
+__device__ __forceinline__ bool bar_wait(uint64_t* b, uint32_t parity, volatile int* lost) {
+  if (bar_try<CLUSTER>(b, parity)) return true;
+  for (uint32_t i = 1; i < kPolls; ++i) {
+    if (bar_try<CLUSTER>(b, parity)) return true;
+    if ((i & 255u) == 0 && *lost) return false;
   }
   *lost = 1;
   return false;
 }
-// the same for a barrier that other CTAs of the cluster arrive on
-__device__ __forceinline__ bool bar_wait_cluster(uint64_t* b, uint32_t parity, volatile int* lost) {
-  const uint32_t limit = *lost ? kPollsLost : kPolls;
-  for (uint32_t i = 0; i < limit; ++i) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(s32(b)), "r"(parity)
-        : "memory");
-    if (ok) return true;
-  }
-  *lost = 1;
-  return false;
+// both phases; the tries overlap
+__device__ __forceinline__ bool bar_wait2(uint64_t* b, uint32_t pb, uint64_t* c, uint32_t pc, volatile int* lost) {
+  const bool b1 = bar_try<false>(b, pb), c1 = bar_try<false>(c, pc);
+  if (b1 && c1) return true;
+  const bool b2 = b1 || bar_wait(b, pb, lost);
+  return (c1 || bar_wait(c, pc, lost)) && b2;
 }
 __device__ __forceinline__ uint32_t peer(const void* local, uint32_t rank) {
   uint32_t r;
