@@ -23,12 +23,22 @@
 
 namespace llx {
 
+// SMALL: step < 2^28, so e stays in 32 bits (g is below 2^16).
+template <bool SMALL>
 __device__ __forceinline__ uint32_t gap_weight(uint32_t g, uint64_t step, const uint32_t* pow2) {
-  const uint64_t e = (g * step) >> 12;
-  const uint64_t n = e >> 20;
-  if (n >= 32) return 0;
-  const uint32_t b = pow2[(uint32_t)(e >> 10) & 1023u];
-  return (b - __umulhi(b, ((uint32_t)e & 1023u) * 2839u)) >> (uint32_t)n;
+  uint32_t e, n;
+  if (SMALL) {
+    e = (uint32_t)(((uint64_t)g * (uint32_t)step) >> 12);
+    n = e >> 20;
+  } else {
+    const uint64_t x = (g * step) >> 12;
+    e = (uint32_t)x;
+    n = x >> 20 < 32 ? (uint32_t)(x >> 20) : 32u;
+  }
+  const uint32_t b = pow2[(e >> 10) & 1023u];
+  uint32_t w;
+  asm("shr.u32 %0, %1, %2;" : "=r"(w) : "r"(b - __umulhi(b, (e & 1023u) * 2839u)), "r"(n));  // 0 from 32 bits on
+  return w;
 }
 
 // floor and ceiling of total * f / 2^31, f <= 2^31
@@ -85,7 +95,8 @@ __device__ __forceinline__ SampleRow sample_row(const llx_sample_args& a, int64_
 // ---------------------------------------------------------------------------------------
 constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kBins = 2 * kThreads;      // two per thread
-constexpr int kMaxCluster = 8;
+constexpr int kFirst = 256;
+constexpr int kMaxCluster = 16;
 constexpr int kSliceVecs = 6400;         // 51,200 tokens: a bin's 16-bit halves of weights stay in 32 bits
 constexpr int kOut = 1 << 20;            // gap of a place that holds no token
 
@@ -111,11 +122,13 @@ __device__ __forceinline__ uint64_t peer_u64(const void* local, int rank) {
 
 struct SampleShared {
   uint32_t count[kBins], low[kBins], high[kBins];  // gaps: tokens, their weights' lower and upper 16 bits
-  uint32_t first[kBins];                           // gaps of the threads' maxima
+  uint64_t added[3][kBins / 4];                    // this CTA's share of the bins, of all CTAs (4 or more)
+  uint32_t first[kFirst];                          // gaps of the threads' maxima, 256 levels a bin
   uint32_t level[2][64];                           // tokens per level of a bin: for top-k, for top-p
   uint32_t pow2[1024];
   uint64_t warp_sum[kWarps];
   uint32_t warp_count[kWarps];
+  SampleRow set;
   // read by the peers
   int32_t max;
   uint64_t whole;
@@ -129,7 +142,8 @@ struct SampleShared {
   int64_t take;
 };
 
-__device__ __forceinline__ void cluster_meet(int C) {
+template <int C>
+__device__ __forceinline__ void cluster_meet() {
   if (C > 1)
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
   else
@@ -166,13 +180,15 @@ __device__ __forceinline__ CountSum block_prefix(CountSum v, SampleShared& sh, C
   return CountSum{before.sum + s.sum - v.sum, before.count + s.count - v.count};
 }
 
-__global__ void __launch_bounds__(kThreads, 2) k_sample(const llx_sample_args a, const int C, const int slice) {
+template <int C>
+__global__ void __launch_bounds__(kThreads, 2) k_sample(const llx_sample_args a, const int slice) {
   extern __shared__ __align__(16) uint4 vecs[];  // this CTA's part of the row
   __shared__ SampleShared sh;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t r = blockIdx.x / C;
   const int rank = (int)(blockIdx.x % C);
-  for (int x = tid; x < kBins; x += kThreads) sh.count[x] = sh.low[x] = sh.high[x] = sh.first[x] = 0;
+  for (int x = tid; x < kBins; x += kThreads) sh.count[x] = sh.low[x] = sh.high[x] = 0;
+  if (tid < kFirst) sh.first[tid] = 0;
   for (int x = tid; x < 1024; x += kThreads) sh.pow2[x] = kDevPow2[x];
   if (tid < 64) sh.level[0][tid] = sh.level[1][tid] = 0;
   pdl_trigger();
@@ -196,7 +212,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const llx_sample_args a,
       for (int j = 0; j < 8; ++j) mine = max(mine, (int)e[j]);
       any = true;
     } else {
-      x = make_uint4(0, 0, 0, 0);
+      x = make_uint4(0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u);
 #pragma unroll
       for (int j = 0; j < 8; ++j)
         if (v * 8 + j >= lo && v * 8 + j < hi) {
@@ -207,19 +223,21 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const llx_sample_args a,
     }
     vecs[v] = x;
   }
-  const SampleRow set = sample_row(a, r);
+  // one thread works out the row's settings (doubles) while the others load
+  if (tid == kThreads - 1) sh.set = sample_row(a, r);
   {
     const int m = __reduce_max_sync(0xffffffffu, any ? mine : INT_MIN);
     if (lane == 0) sh.warp_count[warp] = (uint32_t)m;
     __syncthreads();
-    if (tid == 0) {
-      int x = INT_MIN;
-      for (int w = 0; w < kWarps; ++w) x = max(x, (int)sh.warp_count[w]);
-      sh.max = x;
+    if (warp == 0) {
+      const int x = __reduce_max_sync(0xffffffffu, lane < kWarps ? (int)sh.warp_count[lane] : INT_MIN);
+      if (lane == 0) sh.max = x;
     }
   }
-  cluster_meet(C);
+  cluster_meet<C>();
+  const SampleRow set = sh.set;
   int mx = INT_MIN;
+#pragma unroll
   for (int c = 0; c < C; ++c) mx = max(mx, C > 1 ? (int)peer_u32(&sh.max, c) : sh.max);
 
   // the 8 gaps of a vector; places without a token get kOut
@@ -237,15 +255,26 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const llx_sample_args a,
         if (v * 8 + j < lo || v * 8 + j >= hi) g[j] = kOut;
     }
   };
-  auto weight = [&](int g) { return gap_weight((uint32_t)g, set.step, sh.pow2); };
-  auto farthest = [&](uint32_t least) {  // largest gap whose weight is at least `least` (weight(0) is)
-    int l = 0, h = 65536;
-    while (h - l > 1) {
-      const int mid = (l + h) >> 1;
-      if (weight(mid) >= least)
-        l = mid;
-      else
-        h = mid;
+  // whether a vector has a token within `reach`: the largest of its places first, two at a time
+  auto near = [&](int v, int reach) {
+    const uint4 x = vecs[v];
+    const uint32_t m = __vmaxs2(__vmaxs2(x.x, x.y), __vmaxs2(x.z, x.w));
+    return mx - max((int)(int16_t)(m & 0xffffu), (int)m >> 16) <= reach;
+  };
+  const bool small = set.step < (1ull << 28);
+  auto weight = [&](int g) {
+    return small ? gap_weight<true>((uint32_t)g, set.step, sh.pow2) : gap_weight<false>((uint32_t)g, set.step, sh.pow2);
+  };
+  // largest gap whose weight is at least `least` (weight(0) is): every warp tries 32 gaps a round
+  auto farthest = [&](uint32_t least) {
+    int l = 0;
+#pragma unroll 1
+    for (int width = 2048;; width >>= 5) {  // 2048, 64, 2, 1
+      if (width == 0) width = 1;
+      const int g = l + lane * width;
+      const uint32_t ok = __ballot_sync(0xffffffffu, g < 65536 && weight(g) >= least);
+      l += (__popc(ok) - 1) * width;
+      if (width == 1) break;
     }
     return l;
   };
@@ -257,20 +286,19 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const llx_sample_args a,
     int reach = 65535;  // no token beyond this gap matters
     if (by_k) {
       if (set.k <= (int64_t)kThreads * C) {
-        if (any) atomicAdd(&sh.first[min((mx - mine) >> 6, kBins - 1)], 1u);
-        cluster_meet(C);
-        uint32_t n0 = 0, n1 = 0;
-        for (int c = 0; c < C; ++c) {
-          n0 += C > 1 ? peer_u32(&sh.first[2 * tid], c) : sh.first[2 * tid];
-          n1 += C > 1 ? peer_u32(&sh.first[2 * tid + 1], c) : sh.first[2 * tid + 1];
-        }
+        if (any) atomicAdd(&sh.first[(mx - mine) >> 8], 1u);
+        cluster_meet<C>();
+        uint32_t n = 0;
+        if (tid < kFirst)
+#pragma unroll
+          for (int c = 0; c < C; ++c) n += C > 1 ? peer_u32(&sh.first[tid], c) : sh.first[tid];
         CountSum all;
-        const CountSum at = block_prefix(CountSum{0, n0 + n1}, sh, &all);
-        if (tid == 0) sh.bin[2] = kBins - 1;
+        const CountSum at = block_prefix(CountSum{0, n}, sh, &all);
+        if (tid == 0) sh.bin[2] = kFirst - 1;
         __syncthreads();
-        if (at.count < set.k && at.count + n0 + n1 >= set.k) sh.bin[2] = at.count + n0 >= set.k ? 2 * tid : 2 * tid + 1;
+        if (at.count < set.k && at.count + n >= set.k) sh.bin[2] = tid;
         __syncthreads();
-        if (sh.bin[2] < kBins - 1) reach = sh.bin[2] * 64 + 63;
+        reach = sh.bin[2] * 256 + 255;
       }
     } else {
       uint64_t sum = 0;
@@ -284,8 +312,9 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const llx_sample_args a,
       CountSum all;
       block_prefix(CountSum{sum, 0}, sh, &all);
       if (tid == 0) sh.whole = all.sum;
-      cluster_meet(C);
+      cluster_meet<C>();
       uint64_t whole = 0;
+#pragma unroll
       for (int c = 0; c < C; ++c) whole += C > 1 ? peer_u64(&sh.whole, c) : sh.whole;
       const uint64_t need = max(part_ceil(whole, set.part), (uint64_t)1);
       const uint64_t light = (whole - need) / (uint64_t)V;
@@ -295,13 +324,14 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const llx_sample_args a,
     int s = 0;
     while ((reach >> s) >= kBins) ++s;
     for (int v = tid; v < nv; v += kThreads) {
+      if (!near(v, reach)) continue;
       int g[8];
       gaps(v, g);
 #pragma unroll
       for (int j = 0; j < 8; ++j)
         if (g[j] <= reach) {
           const int b = g[j] >> s;
-          atomicAdd(&sh.count[b], 1u);
+          if (by_k) atomicAdd(&sh.count[b], 1u);
           if (set.by_part) {
             const uint32_t w = weight(g[j]);
             atomicAdd(&sh.low[b], w & 0xffffu);
@@ -309,16 +339,37 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const llx_sample_args a,
           }
         }
     }
-    cluster_meet(C);
+    cluster_meet<C>();
     CountSum bin[2] = {{0, 0}, {0, 0}}, all;
-    for (int c = 0; c < C; ++c)
+    if constexpr (C <= 2) {
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const int b = 2 * tid + x;
+          bin[x].count += C > 1 ? peer_u32(&sh.count[b], c) : sh.count[b];
+          bin[x].sum += (C > 1 ? peer_u32(&sh.low[b], c) : sh.low[b]) + ((uint64_t)(C > 1 ? peer_u32(&sh.high[b], c) : sh.high[b]) << 16);
+        }
+    } else {
+      // every CTA adds up its share of the bins, then all read the sums: 2 x 24 KB over the cluster's
+      // network where reading all of every peer's bins would be C x 12
+      constexpr int kShare = kBins / C;
+#pragma unroll
+      for (int x = tid; x < 3 * kShare; x += kThreads) {
+        const uint32_t* from = (x < kShare ? sh.count : x < 2 * kShare ? sh.low : sh.high) + rank * kShare + x % kShare;
+        uint64_t n = 0;
+#pragma unroll
+        for (int c = 0; c < C; ++c) n += peer_u32(from, c);
+        sh.added[x / kShare][x % kShare] = n;
+      }
+      cluster_meet<C>();
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        const int b = 2 * tid + x;
-        bin[x].count += C > 1 ? peer_u32(&sh.count[b], c) : sh.count[b];
-        if (set.by_part)
-          bin[x].sum += (C > 1 ? peer_u32(&sh.low[b], c) : sh.low[b]) + ((uint64_t)(C > 1 ? peer_u32(&sh.high[b], c) : sh.high[b]) << 16);
+        const int b = 2 * tid + x, c = b / kShare;
+        bin[x].count = (uint32_t)peer_u64(&sh.added[0][b % kShare], c);
+        bin[x].sum = peer_u64(&sh.added[1][b % kShare], c) + (peer_u64(&sh.added[2][b % kShare], c) << 16);
       }
+    }
     const CountSum at = block_prefix(CountSum{bin[0].sum + bin[1].sum, bin[0].count + bin[1].count}, sh, &all);
     // The cut of kind q (0: top-k by count, 1: top-p by weight) among the tokens of its bin, level by
     // level: the first level at which `enough` holds of what is below and within.
@@ -337,18 +388,20 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const llx_sample_args a,
       __syncthreads();
       const int b = sh.bin[q];
       for (int v = tid; v < nv; v += kThreads) {
+        if (!near(v, ((b + 1) << s) - 1)) continue;
         int g[8];
         gaps(v, g);
 #pragma unroll
         for (int j = 0; j < 8; ++j)
           if (g[j] >> s == b) atomicAdd(&sh.level[q][g[j] - (b << s)], 1u);
       }
-      cluster_meet(C);
+      cluster_meet<C>();
       if (warp == 0) {
         CountSum lv[2] = {{0, 0}, {0, 0}};
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           const int l = 2 * lane + x;
+#pragma unroll
           for (int c = 0; c < C; ++c) lv[x].count += C > 1 ? peer_u32(&sh.level[q][l], c) : sh.level[q][l];
           if (lv[x].count) lv[x].sum = (uint64_t)lv[x].count * weight((b << s) + l);
         }
@@ -387,6 +440,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const llx_sample_args a,
     if (set.by_part) {
       if (!by_k) {
         total = 0;
+#pragma unroll
         for (int c = 0; c < C; ++c) total += C > 1 ? peer_u64(&sh.whole, c) : sh.whole;
       }
       const uint64_t need = max(part_ceil(total, set.part), (uint64_t)1);
@@ -404,122 +458,129 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const llx_sample_args a,
   }
   // ---- kept weights in index order: a segment of the slice per warp, then the draw ----
   const uint32_t wG = weight(G);
-  const int seg = (nv + kWarps - 1) / kWarps, s0 = min(nv, warp * seg), s1 = min(nv, s0 + seg);
+  // a thread's vectors follow one another, an odd number of them: 16-byte reads of neighbouring threads
+  // then hit different banks
+  const int chunk = ((nv + kThreads - 1) / kThreads) | 1, c0 = min(nv, tid * chunk), c1 = min(nv, c0 + chunk);
   auto kept = [&](int v, int (&g)[8]) {
     CountSum t{0, 0};
-    if (v < s1) gaps(v, g);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) g[j] = kOut;
+    if (!near(v, G)) return t;
+    gaps(v, g);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      if (v >= s1) g[j] = kOut;
       if (g[j] < G) t.sum += weight(g[j]);
       t.count += g[j] == G;
     }
     return t;
   };
   CountSum own{0, 0};
-  for (int v = s0 + lane; v - lane < s1; v += 32) {
+  for (int v = c0; v < c1; ++v) {
     int g[8];
     const CountSum t = kept(v, g);
     own.sum += t.sum;
     own.count += t.count;
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    own.sum += __shfl_xor_sync(0xffffffffu, own.sum, o);
-    own.count += __shfl_xor_sync(0xffffffffu, own.count, o);
-  }
-  __syncthreads();
-  if (lane == 0) {
-    sh.warp_sum[warp] = own.sum;
-    sh.warp_count[warp] = own.count;
-  }
-  __syncthreads();
+  CountSum here;  // this CTA's
+  const CountSum ahead = block_prefix(own, sh, &here);
   if (tid == 0) {
-    uint64_t x = 0;
-    uint32_t n = 0;
-    for (int w = 0; w < kWarps; ++w) {
-      x += sh.warp_sum[w];
-      n += sh.warp_count[w];
-    }
-    sh.kept = x;
-    sh.ties = n;
+    sh.kept = here.sum;
+    sh.ties = here.count;
   }
-  cluster_meet(C);
+  cluster_meet<C>();
   CountSum before{0, 0}, all{0, 0};
+#pragma unroll
   for (int c = 0; c < C; ++c) {
     if (c == rank) before = all;
     all.sum += C > 1 ? peer_u64(&sh.kept, c) : sh.kept;
     all.count += C > 1 ? peer_u32(&sh.ties, c) : sh.ties;
   }
-  for (int w = 0; w < warp; ++w) {
-    before.sum += sh.warp_sum[w];
-    before.count += sh.warp_count[w];
-  }
+  before.sum += ahead.sum;
+  before.count += ahead.count;
   const int64_t ties = min(take, (int64_t)all.count);
   const uint64_t total = all.sum + (uint64_t)ties * wG, target = part_floor(total, set.u);
   // running kept weight once `sum` of lesser gaps and `n` ties have gone by
   auto run_at = [&](uint64_t sum, int64_t n) { return sum + (uint64_t)min(n, ties) * wG; };
-  const uint64_t first = run_at(before.sum, before.count), last = run_at(before.sum + own.sum, (int64_t)before.count + own.count);
-  if (first <= target && target < last) {  // one warp of one CTA: its segment has the token
-    for (int v = s0 + lane; v - lane < s1; v += 32) {
-      int g[8];
-      const CountSum t = kept(v, g);
-      CountSum e = t;
+  const bool has = run_at(before.sum, before.count) <= target &&
+                   target < run_at(before.sum + own.sum, (int64_t)before.count + own.count);
+  const uint32_t who = __ballot_sync(0xffffffffu, has);
+  if (who) {  // one thread of one CTA has the token: its vectors, one per lane (a slice has at most 13 a thread)
+    const int l = __ffs(who) - 1, v = __shfl_sync(0xffffffffu, c0, l) + lane;
+    CountSum w{__shfl_sync(0xffffffffu, before.sum, l), __shfl_sync(0xffffffffu, before.count, l)};
+    int g[8];
+    CountSum t{0, 0};
+    const bool in = v < __shfl_sync(0xffffffffu, c1, l);
+    if (in) t = kept(v, g);
+    CountSum e = t;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint64_t ys = __shfl_up_sync(0xffffffffu, e.sum, o);
-        const uint32_t yc = __shfl_up_sync(0xffffffffu, e.count, o);
-        if (lane >= o) {
-          e.sum += ys;
-          e.count += yc;
-        }
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint64_t ys = __shfl_up_sync(0xffffffffu, e.sum, o);
+      const uint32_t yc = __shfl_up_sync(0xffffffffu, e.count, o);
+      if (lane >= o) {
+        e.sum += ys;
+        e.count += yc;
       }
-      uint64_t sum = before.sum + e.sum - t.sum;
-      int64_t n = (int64_t)before.count + e.count - t.count;
-#pragma unroll
+    }
+    w.sum += e.sum - t.sum;
+    w.count += e.count - t.count;
+    if (in && run_at(w.sum, w.count) <= target && target < run_at(w.sum + t.sum, (int64_t)w.count + t.count)) {
+      int64_t n = w.count;
+#pragma unroll 1
       for (int j = 0; j < 8; ++j) {
-        const uint64_t start = run_at(sum, n);
-        if (g[j] < G) sum += weight(g[j]);
-        n += g[j] == G;
-        const uint64_t end = run_at(sum, n);
+        const int x = mx - (int)reinterpret_cast<const int16_t*>(vecs)[v * 8 + j];
+        if (v * 8 + j < lo || v * 8 + j >= hi) continue;
+        const uint64_t start = run_at(w.sum, n);
+        if (x < G) w.sum += weight(x);
+        n += x == G;
+        const uint64_t end = run_at(w.sum, n);
         if (start <= target && target < end) {
           a.token[r] = (v0 + v) * 8 + j - skew;
           if (a.prob) a.prob[r] = (float)((double)(end - start) / (double)total);
         }
       }
-      before.sum += __shfl_sync(0xffffffffu, e.sum, 31);
-      before.count += __shfl_sync(0xffffffffu, e.count, 31);
     }
   }
   if (C > 1) {  // no CTA leaves while a peer may still read from it
     __syncwarp();
-    cluster_meet(C);
+    cluster_meet<C>();
   }
 }
 
 int64_t sample_max_vocab() { return 1ll << 18; }
 
-cudaError_t launch_sample(const llx_sample_args& a, cudaStream_t st) {
-  if (a.rows == 0) return cudaSuccess;
+template <int C>
+static cudaError_t launch_sample_t(const llx_sample_args& a, int slice, cudaStream_t st) {
   static std::atomic<bool> ready[64];
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
   if (!ready[dev].load(std::memory_order_acquire)) {
-    e = cudaFuncSetAttribute(k_sample, cudaFuncAttributeMaxDynamicSharedMemorySize, kSliceVecs * 16);
+    e = cudaFuncSetAttribute(k_sample<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSliceVecs * 16);
+    if (e == cudaSuccess && C > 8) e = cudaFuncSetAttribute(k_sample<C>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return e;
     ready[dev].store(true, std::memory_order_release);
   }
+  const dim3 grid((unsigned)(a.rows * C));
+  if (C == 1) return launch_k(k_sample<C>, grid, dim3(kThreads), (size_t)slice * 16, st, a, slice);
+  return launch_kc(k_sample<C>, grid, dim3(kThreads), (size_t)slice * 16, st, dim3(C, 1, 1), a, slice);
+}
+
+cudaError_t launch_sample(const llx_sample_args& a, cudaStream_t st) {
+  if (a.rows == 0) return cudaSuccess;
   // Split a row until two CTAs per SM have work, as long as a CTA keeps a vector per thread; and where
   // a slice would not fit.
   const int64_t vecs = (a.vocab + 14) / 8;  // from any alignment
   int C = 1;
   while (C < kMaxCluster && ((a.rows * C < 2 * 148 && vecs > (int64_t)C * kThreads) || vecs > (int64_t)C * kSliceVecs)) C *= 2;
   const int slice = (int)((vecs + C - 1) / C);
-  const dim3 grid((unsigned)(a.rows * C));
-  if (C == 1) return launch_k(k_sample, grid, dim3(kThreads), (size_t)slice * 16, st, a, C, slice);
-  return launch_kc(k_sample, grid, dim3(kThreads), (size_t)slice * 16, st, dim3(C, 1, 1), a, C, slice);
+  switch (C) {
+    case 1: return launch_sample_t<1>(a, slice, st);
+    case 2: return launch_sample_t<2>(a, slice, st);
+    case 4: return launch_sample_t<4>(a, slice, st);
+    case 8: return launch_sample_t<8>(a, slice, st);
+    default: return launch_sample_t<16>(a, slice, st);
+  }
 }
 
 }  // namespace llx

@@ -202,7 +202,7 @@ llx_status llx_sample(const llx_sample_args* args, void* stream) {
   return call(
       "llx_sample", args, stream,
       [](const llx_sample_args& a) {
-        need(a.rows >= 0 && a.rows < (1ll << 30), "rows must be 0 to 2^30");
+        need(a.rows >= 0 && a.rows <= (1ll << 26), "rows must be 0 to 2^26");
         need(a.vocab >= 1, "an empty vocabulary");
         need(a.vocab <= sample_max_vocab(), "the vocabulary exceeds 262144 tokens", LLX_ERR_UNSUPPORTED);
         need(a.logits_stride >= a.vocab, "the row stride is smaller than the vocabulary");
