@@ -13,38 +13,56 @@ namespace llx {
 // ---------------------------------------------------------------------------------------
 // Append: per row and head, RMSNorm over the head (numerics.h:60-71), rotation at the row's
 // position (numerics.h:75-84) and requantization; queries to q8, keys and values to the page
-// of their position.  One block per row, one warp per head at a time.
+// of their position.
 // ---------------------------------------------------------------------------------------
-__global__ void __launch_bounds__(256) k_paged_append(const llx_paged_append_args a) {
+
+// Where a launch row goes: its position and page, or a status code.
+struct Place {
+  int64_t pos, page;
+  int code;
+  bool absent;  // behind the last sequence
+};
+__device__ __forceinline__ Place place_row(const llx_paged_append_args& a, int r) {
+  Place p{-1, -1, 0, false};
+  const int i = find_sequence(a.q_start, (int)a.n_seqs, r);
+  if (i < 0) {
+    p.absent = true;
+    return p;
+  }
+  const int slot = a.seqs ? a.seqs[i] : i;
+  if (slot < 0 || slot >= a.max_seqs) {
+    p.code = LLX_STATUS_BAD_SLOT;
+    return p;
+  }
+  p.pos = (int64_t)a.length[slot] - (a.q_start[i + 1] - r);
+  const int shift = __ffs((int)a.page_size) - 1;
+  if (p.pos < 0 || p.pos >= a.n_positions || p.pos >> shift >= a.max_pages) {
+    p.code = LLX_STATUS_BAD_POSITION;
+    return p;
+  }
+  p.page = a.table[slot * a.table_stride + (p.pos >> shift)];
+  if (p.page < 0 || p.page >= a.n_pages) p.code = LLX_STATUS_BAD_PAGE;
+  return p;
+}
+
+// Any geometry, constants and alignment: one block per row, one warp per head at a time.
+__global__ void __launch_bounds__(256) k_paged_append_any(const llx_paged_append_args a) {
   pdl_trigger();
   pdl_wait();
   const int r = blockIdx.x;
-  const int i = find_sequence(a.q_start, (int)a.n_seqs, r);
-  if (i < 0) return;
-  const int slot = a.seqs ? a.seqs[i] : i;
+  const Place at = place_row(a, r);
+  if (at.absent) return;
   const int D = (int)a.head_dim, half = D / 2, H = (int)a.n_heads, Hkv = (int)a.n_kv_heads;
-  int64_t pos = -1;
-  int page = -1, code = 0;
-  if (slot < 0 || slot >= a.max_seqs) {
-    code = LLX_STATUS_BAD_SLOT;
-  } else {
-    pos = (int64_t)a.length[slot] - (a.q_start[i + 1] - r);
-    if (pos < 0 || pos >= a.n_positions || pos >= a.max_pages * a.page_size) {
-      code = LLX_STATUS_BAD_POSITION;
-    } else {
-      page = a.table[slot * a.table_stride + pos / a.page_size];
-      if (page < 0 || page >= a.n_pages) code = LLX_STATUS_BAD_PAGE;
-    }
-  }
+  const int64_t pos = at.pos, page = at.page;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   int8_t* q8 = a.q8 + r * a.q8_stride;
-  if (code) {
-    if (threadIdx.x == 0) raise_status(a.status, code);
+  if (at.code) {
+    if (threadIdx.x == 0) raise_status(a.status, at.code);
     for (int e = threadIdx.x; e < H * D; e += blockDim.x) q8[e] = 0;
     return;
   }
   const int row = (int)(pos % a.page_size);
-  const int64_t head0 = (int64_t)page * a.page_stride + (int64_t)row * D;  // key / value row of head 0
+  const int64_t head0 = page * a.page_stride + (int64_t)row * D;  // key / value row of head 0
   const int64_t head_step = a.page_size * D;
   const int16_t* ct = a.cos + pos * half;
   const int16_t* sn = a.sin + pos * half;
@@ -82,9 +100,180 @@ __global__ void __launch_bounds__(256) k_paged_append(const llx_paged_append_arg
   for (int e = threadIdx.x; e < Hkv * D; e += blockDim.x) a.v_pages[head0 + (e / D) * head_step + e % D] = v[e];
 }
 
+// The usual case: head_dim D a power of two, 16-byte aligned rows, multipliers below 2^31 with shifts
+// of 32 and more (how the quantizer normalises them), norm shifts of 18 to 46.  D / 16 lanes share a
+// head, each with 8 neighbouring values and their 8 partners half a head away: one 16-byte load each,
+// and a rotation without exchange.  The row's place is looked up while those loads are under way.
+// Bytes bound it: per row 2 (H + Hkv) D + Hkv D read, H D + 2 Hkv D written.
+struct AppendSide {
+  const int16_t *x, *gamma;
+  int64_t eps, C, stride;
+  int shift;
+  int32_t M;
+  int S;
+};
+
+__device__ __forceinline__ void unpack8(const uint4& v, int (&x)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    x[2 * j] = (int)(int16_t)(w[j] & 0xffffu);
+    x[2 * j + 1] = (int)w[j] >> 16;
+  }
+}
+__device__ __forceinline__ int clamp32(int v, int lo, int hi) { return max(lo, min(hi, v)); }
+
+// floor(sqrt(t)) for t < 2^48: a float root is off by less than 2, integer products settle it
+__device__ __forceinline__ uint32_t root48(uint64_t t) {
+  uint32_t r = (uint32_t)sqrtf((float)t);
+  while ((uint64_t)r * r > t) --r;
+  while ((uint64_t)(r + 1) * (r + 1) <= t) ++r;
+  return r;
+}
+// min(65535, C / r) for C < 2^40, 1 <= r < 2^24: below 2^17 a float quotient is off by less than 1
+__device__ __forceinline__ uint32_t inverse16(uint64_t C, uint32_t r) {
+  const float f = (float)C / (float)r;
+  uint32_t q = f >= 65536.0f ? 65536u : (uint32_t)f;
+  while ((uint64_t)q * r > C) --q;
+  while (q < 65536u && (uint64_t)(q + 1) * r <= C) ++q;
+  return q < 65535u ? q : 65535u;
+}
+
+// two 32-bit values saturated to 8 bits, above the lower two bytes of `rest`
+__device__ __forceinline__ uint32_t pack_sat8(int b, int a, uint32_t rest) {
+  uint32_t d;
+  asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, %3;" : "=r"(d) : "r"(b), "r"(a), "r"(rest));
+  return d;
+}
+
+template <int D>
+__global__ void __launch_bounds__(128) k_paged_append(const llx_paged_append_args a, const AppendSide sq, const AppendSide sk,
+                                                      const int parts, const int warps_per_row) {
+  constexpr int L = D / 16, kHalf = D / 2;  // lanes per head
+  pdl_trigger();
+  pdl_wait();
+  const int64_t w = blockIdx.x * 4ll + (threadIdx.x >> 5);
+  const int r = (int)(w / warps_per_row), first = (int)(w - (int64_t)r * warps_per_row);
+  if (r >= a.rows) return;
+  const int lane = threadIdx.x & 31;
+  const int H = (int)a.n_heads, Hkv = (int)a.n_kv_heads;
+  // 32 lanes' worth of the row's heads and values at a time
+  auto fetch = [&](int task, uint4& lo, uint4& hi) {
+    const int h = task / L, sub = task % L;
+    lo = hi = make_uint4(0, 0, 0, 0);
+    if (h < H + Hkv) {
+      const AppendSide& s = h < H ? sq : sk;
+      const int16_t* x = s.x + r * s.stride + (int64_t)(h < H ? h : h - H) * D + sub * 8;
+      lo = *reinterpret_cast<const uint4*>(x);
+      hi = *reinterpret_cast<const uint4*>(x + kHalf);
+    } else if (task < (H + 2 * Hkv) * L) {
+      lo = *reinterpret_cast<const uint4*>(a.v + r * a.v_stride + (task - (H + Hkv) * L) * 16);
+    }
+  };
+  uint4 lo, hi;
+  fetch(first * 32 + lane, lo, hi);
+  const Place at = place_row(a, r);
+  if (at.absent) return;
+  int8_t* q8 = a.q8 + r * a.q8_stride;
+  if (at.code && first == 0 && lane == 0) raise_status(a.status, at.code);
+  const int P = (int)a.page_size, prow = (int)at.pos & (P - 1);
+  const int64_t page0 = at.page * a.page_stride + (int64_t)prow * D;  // row of head 0
+  for (int part = first; part < parts; part += warps_per_row) {
+    const int task = part * 32 + lane, h = task / L, sub = task % L;
+    const bool rotates = h < H + Hkv, is_q = h < H;
+    const AppendSide& s = is_q ? sq : sk;
+    const int hh = is_q ? h : h - H, vtask = task - (H + Hkv) * L;
+    uint4 next_lo, next_hi;
+    fetch((part + warps_per_row) * 32 + lane, next_lo, next_hi);
+    if (at.code) {
+      if (is_q) *reinterpret_cast<uint4*>(q8 + (int64_t)hh * D + sub * 16) = make_uint4(0, 0, 0, 0);
+      continue;
+    }
+    int x1[8], x2[8];
+    unpack8(lo, x1);
+    unpack8(hi, x2);
+    if (sq.gamma || sk.gamma) {  // lanes of queries, keys and values share a warp: all take part in the sums
+      uint64_t ss = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) ss += (uint64_t)((int64_t)x1[j] * x1[j]) + (uint64_t)((int64_t)x2[j] * x2[j]);
+#pragma unroll
+      for (int o = 1; o < L; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      if (rotates && s.gamma) {
+        const uint32_t root = root48(ss + (uint64_t)s.eps);
+        // |x g inv| < 2^46: 14 bits more keep it in 64 and put the result into the upper word
+        const int inv = (int)(inverse16((uint64_t)s.C, root ? root : 1u) << 14), sh = s.shift + 14 - 32;
+        int g1[8], g2[8];
+        unpack8(*reinterpret_cast<const uint4*>(s.gamma + sub * 8), g1);
+        unpack8(*reinterpret_cast<const uint4*>(s.gamma + kHalf + sub * 8), g2);
+        const int64_t half = 1ll << (s.shift + 13);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          x1[j] = clamp32((int)(((int64_t)(x1[j] * g1[j]) * inv + half) >> 32) >> sh, -32768, 32767);
+          x2[j] = clamp32((int)(((int64_t)(x2[j] * g2[j]) * inv + half) >> 32) >> sh, -32768, 32767);
+        }
+      }
+    }
+    if (rotates) {
+      int c[8], n[8];
+      unpack8(*reinterpret_cast<const uint4*>(a.cos + at.pos * kHalf + sub * 8), c);
+      unpack8(*reinterpret_cast<const uint4*>(a.sin + at.pos * kHalf + sub * 8), n);
+      const int64_t half = 1ll << (s.S - 1);
+      const int sh = s.S - 32;
+      uint32_t o1[2], o2[2];
+      int z1[8], z2[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        // of 16-bit values x1 c - x2 s stays in 32 bits with the rounding; x2 c + x1 s can be 2^31
+        const int y1 = clamp32((x1[j] * c[j] - x2[j] * n[j] + 8192) >> 14, -32768, 32767);
+        const int y2 = clamp32((int)(((int64_t)x2[j] * c[j] + (int64_t)x1[j] * n[j] + 8192) >> 14), -32768, 32767);
+        z1[j] = (int)(((int64_t)y1 * s.M + half) >> 32) >> sh;
+        z2[j] = (int)(((int64_t)y2 * s.M + half) >> 32) >> sh;
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        o1[j] = pack_sat8(z1[4 * j + 1], z1[4 * j], pack_sat8(z1[4 * j + 3], z1[4 * j + 2], 0));
+        o2[j] = pack_sat8(z2[4 * j + 1], z2[4 * j], pack_sat8(z2[4 * j + 3], z2[4 * j + 2], 0));
+      }
+      int8_t* dst = is_q ? q8 + (int64_t)hh * D : a.k_pages + page0 + (int64_t)hh * P * D;
+      *reinterpret_cast<uint2*>(dst + sub * 8) = make_uint2(o1[0], o1[1]);
+      *reinterpret_cast<uint2*>(dst + kHalf + sub * 8) = make_uint2(o2[0], o2[1]);
+    } else if (vtask < Hkv * L) {
+      *reinterpret_cast<uint4*>(a.v_pages + page0 + (int64_t)(vtask / L) * P * D + (vtask % L) * 16) = lo;
+    }
+    lo = next_lo;
+    hi = next_hi;
+  }
+}
+
+template <int D>
+static cudaError_t launch_append_t(const llx_paged_append_args& a, const AppendSide& q, const AppendSide& k, cudaStream_t st) {
+  const int64_t parts = ((a.n_heads + 2 * a.n_kv_heads) * (D / 16) + 31) / 32;
+  // with many rows a warp takes two parts of one: the row's place is looked up once for both
+  const int64_t per_row = a.rows * parts > 148 * 64 ? (parts + 1) / 2 : parts;
+  const int64_t blocks = (a.rows * per_row + 3) / 4;
+  if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
+  return launch_k(k_paged_append<D>, dim3((unsigned)blocks), dim3(128), 0, st, a, q, k, (int)parts, (int)per_row);
+}
+
 cudaError_t launch_paged_append(const llx_paged_append_args& a, cudaStream_t st) {
   if (a.rows == 0 || a.n_seqs == 0) return cudaSuccess;
-  return launch_k(k_paged_append, dim3((unsigned)a.rows), dim3(256), 0, st, a);
+  const AppendSide q{a.q, a.q_gamma, a.q_eps, a.q_C, a.q_stride, (int)a.q_shift, (int32_t)a.q_M, (int)a.q_S};
+  const AppendSide k{a.k, a.k_gamma, a.k_eps, a.k_C, a.k_stride, (int)a.k_shift, (int32_t)a.k_M, (int)a.k_S};
+  const void* ptrs[] = {a.q, a.k, a.v, a.q8, a.q_gamma, a.k_gamma, a.cos, a.sin, a.k_pages, a.v_pages};
+  bool usual = a.q_stride % 8 == 0 && a.k_stride % 8 == 0 && a.v_stride % 16 == 0 && a.q8_stride % 16 == 0;
+  for (const void* p : ptrs) usual = usual && (reinterpret_cast<uintptr_t>(p) & 15) == 0;
+  for (const AppendSide* s : {&q, &k}) {
+    usual = usual && s->S >= 32 && (s == &q ? a.q_M : a.k_M) < (1ll << 31);
+    if (s->gamma) usual = usual && s->shift >= 18 && s->shift <= 46;
+  }
+  if (usual) switch (a.head_dim) {
+      case 16: return launch_append_t<16>(a, q, k, st);
+      case 32: return launch_append_t<32>(a, q, k, st);
+      case 64: return launch_append_t<64>(a, q, k, st);
+      case 128: return launch_append_t<128>(a, q, k, st);
+      case 256: return launch_append_t<256>(a, q, k, st);
+    }
+  return launch_k(k_paged_append_any, dim3((unsigned)a.rows), dim3(256), 0, st, a);
 }
 
 // ---------------------------------------------------------------------------------------

@@ -23,17 +23,21 @@ int64_t sample_max_vocab();
 
 // ---- device helpers shared by append and attention ------------------------------------------
 // A launch row's place: sequence i with q_start[i] <= r < q_start[i + 1]; -1 behind the last one.
+// A warp's lanes try 32 entries a round: one round of loads for 32 sequences, two for 1024.
 __device__ __forceinline__ int find_sequence(const int32_t* q_start, int n, int r) {
-  if (r >= q_start[n] || r < q_start[0]) return -1;
-  int lo = 0, hi = n;  // q_start[lo] <= r < q_start[hi]
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (q_start[mid] <= r)
-      lo = mid;
-    else
-      hi = mid;
+  const int lane = threadIdx.x & 31;
+  int lo = 0, width = 1;  // entries lo, lo + width, ... are tried; q_start[lo] <= r from the second round on
+  while (width * 32 <= n) width *= 32;
+  for (;;) {
+    const int at = lo + lane * width;
+    const uint32_t below = __ballot_sync(0xffffffffu, at <= n && q_start[at] <= r);
+    if (!below) return -1;
+    // starts ascend, so the tries that are at most r come first
+    lo += (31 - __clz(below)) * width;
+    if (width == 1) break;
+    width /= 32;
   }
-  return lo;
+  return lo < n ? lo : -1;
 }
 
 __device__ __forceinline__ void raise_status(int32_t* status, int code) {
