@@ -148,97 +148,102 @@ __device__ __forceinline__ uint32_t pack_sat8(int b, int a, uint32_t rest) {
 
 template <int D>
 __global__ void __launch_bounds__(128) k_paged_append(const llx_paged_append_args a, const AppendSide sq, const AppendSide sk,
-                                                      const int parts, const int warps_per_row) {
-  constexpr int L = D / 16, kHalf = D / 2;  // lanes per head
+                                                      const int warps_per_row) {
+  constexpr int L = D / 16, kHalf = D / 2, G = 32 / L;  // lanes per head; heads a warp takes at a time
   pdl_trigger();
   pdl_wait();
   const int64_t w = blockIdx.x * 4ll + (threadIdx.x >> 5);
   const int r = (int)(w / warps_per_row), first = (int)(w - (int64_t)r * warps_per_row);
   if (r >= a.rows) return;
-  const int lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, sub = lane % L;
   const int H = (int)a.n_heads, Hkv = (int)a.n_kv_heads;
-  // 32 lanes' worth of the row's heads and values at a time
-  auto fetch = [&](int task, uint4& lo, uint4& hi) {
-    const int h = task / L, sub = task % L;
+  // groups of query heads, then of key heads, then 512-byte pieces of the values
+  const int nq = (H + G - 1) / G, nk = nq + (Hkv + G - 1) / G, groups = nk + (Hkv * D + 511) / 512;
+  auto fetch = [&](int g, uint4& lo, uint4& hi) {
     lo = hi = make_uint4(0, 0, 0, 0);
-    if (h < H + Hkv) {
-      const AppendSide& s = h < H ? sq : sk;
-      const int16_t* x = s.x + r * s.stride + (int64_t)(h < H ? h : h - H) * D + sub * 8;
-      lo = *reinterpret_cast<const uint4*>(x);
-      hi = *reinterpret_cast<const uint4*>(x + kHalf);
-    } else if (task < (H + 2 * Hkv) * L) {
-      lo = *reinterpret_cast<const uint4*>(a.v + r * a.v_stride + (task - (H + Hkv) * L) * 16);
+    if (g < nk) {
+      const bool is_q = g < nq;
+      const int h = (is_q ? g : g - nq) * G + lane / L;
+      if (h < (is_q ? H : Hkv)) {
+        const int16_t* x = (is_q ? sq.x + r * sq.stride : sk.x + r * sk.stride) + (int64_t)h * D + sub * 8;
+        lo = *reinterpret_cast<const uint4*>(x);
+        hi = *reinterpret_cast<const uint4*>(x + kHalf);
+      }
+    } else if (g < groups && (g - nk) * 512 + lane * 16 < Hkv * D) {
+      lo = *reinterpret_cast<const uint4*>(a.v + r * a.v_stride + (g - nk) * 512 + lane * 16);
     }
   };
   uint4 lo, hi;
-  fetch(first * 32 + lane, lo, hi);
+  fetch(first, lo, hi);
   const Place at = place_row(a, r);
   if (at.absent) return;
   int8_t* q8 = a.q8 + r * a.q8_stride;
-  if (at.code && first == 0 && lane == 0) raise_status(a.status, at.code);
+  if (at.code) {
+    if (first == 0 && lane == 0) raise_status(a.status, at.code);
+    for (int x = first * 32 + lane; x < H * L; x += warps_per_row * 32) reinterpret_cast<uint4*>(q8)[x] = make_uint4(0, 0, 0, 0);
+    return;
+  }
   const int P = (int)a.page_size, prow = (int)at.pos & (P - 1);
   const int64_t page0 = at.page * a.page_stride + (int64_t)prow * D;  // row of head 0
-  for (int part = first; part < parts; part += warps_per_row) {
-    const int task = part * 32 + lane, h = task / L, sub = task % L;
-    const bool rotates = h < H + Hkv, is_q = h < H;
-    const AppendSide& s = is_q ? sq : sk;
-    const int hh = is_q ? h : h - H, vtask = task - (H + Hkv) * L;
+  int c[8], n[8];
+  unpack8(*reinterpret_cast<const uint4*>(a.cos + at.pos * kHalf + sub * 8), c);
+  unpack8(*reinterpret_cast<const uint4*>(a.sin + at.pos * kHalf + sub * 8), n);
+  for (int g = first; g < groups; g += warps_per_row) {
     uint4 next_lo, next_hi;
-    fetch((part + warps_per_row) * 32 + lane, next_lo, next_hi);
-    if (at.code) {
-      if (is_q) *reinterpret_cast<uint4*>(q8 + (int64_t)hh * D + sub * 16) = make_uint4(0, 0, 0, 0);
+    fetch(g + warps_per_row, next_lo, next_hi);
+    if (g >= nk) {
+      const int x = (g - nk) * 512 + lane * 16;
+      if (x < Hkv * D) *reinterpret_cast<uint4*>(a.v_pages + page0 + (int64_t)(x / D) * P * D + x % D) = lo;
+      lo = next_lo;
       continue;
     }
+    const bool is_q = g < nq;
+    const AppendSide& s = is_q ? sq : sk;
+    const int h = (is_q ? g : g - nq) * G + lane / L;
     int x1[8], x2[8];
     unpack8(lo, x1);
     unpack8(hi, x2);
-    if (sq.gamma || sk.gamma) {  // lanes of queries, keys and values share a warp: all take part in the sums
+    if (s.gamma) {
       uint64_t ss = 0;
 #pragma unroll
       for (int j = 0; j < 8; ++j) ss += (uint64_t)((int64_t)x1[j] * x1[j]) + (uint64_t)((int64_t)x2[j] * x2[j]);
 #pragma unroll
       for (int o = 1; o < L; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      if (rotates && s.gamma) {
-        const uint32_t root = root48(ss + (uint64_t)s.eps);
-        // |x g inv| < 2^46: 14 bits more keep it in 64 and put the result into the upper word
-        const int inv = (int)(inverse16((uint64_t)s.C, root ? root : 1u) << 14), sh = s.shift + 14 - 32;
-        int g1[8], g2[8];
-        unpack8(*reinterpret_cast<const uint4*>(s.gamma + sub * 8), g1);
-        unpack8(*reinterpret_cast<const uint4*>(s.gamma + kHalf + sub * 8), g2);
-        const int64_t half = 1ll << (s.shift + 13);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          x1[j] = clamp32((int)(((int64_t)(x1[j] * g1[j]) * inv + half) >> 32) >> sh, -32768, 32767);
-          x2[j] = clamp32((int)(((int64_t)(x2[j] * g2[j]) * inv + half) >> 32) >> sh, -32768, 32767);
-        }
-      }
-    }
-    if (rotates) {
-      int c[8], n[8];
-      unpack8(*reinterpret_cast<const uint4*>(a.cos + at.pos * kHalf + sub * 8), c);
-      unpack8(*reinterpret_cast<const uint4*>(a.sin + at.pos * kHalf + sub * 8), n);
-      const int64_t half = 1ll << (s.S - 1);
-      const int sh = s.S - 32;
-      uint32_t o1[2], o2[2];
-      int z1[8], z2[8];
+      const uint32_t root = root48(ss + (uint64_t)s.eps);
+      // |x g inv| < 2^46: 14 bits more keep it in 64 and put the result into the upper word
+      const int inv = (int)(inverse16((uint64_t)s.C, root ? root : 1u) << 14), sh = s.shift + 14 - 32;
+      int g1[8], g2[8];
+      unpack8(*reinterpret_cast<const uint4*>(s.gamma + sub * 8), g1);
+      unpack8(*reinterpret_cast<const uint4*>(s.gamma + kHalf + sub * 8), g2);
+      const int64_t half = 1ll << (s.shift + 13);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        // of 16-bit values x1 c - x2 s stays in 32 bits with the rounding; x2 c + x1 s can be 2^31
-        const int y1 = clamp32((x1[j] * c[j] - x2[j] * n[j] + 8192) >> 14, -32768, 32767);
-        const int y2 = clamp32((int)(((int64_t)x2[j] * c[j] + (int64_t)x1[j] * n[j] + 8192) >> 14), -32768, 32767);
-        z1[j] = (int)(((int64_t)y1 * s.M + half) >> 32) >> sh;
-        z2[j] = (int)(((int64_t)y2 * s.M + half) >> 32) >> sh;
+        x1[j] = clamp32((int)(((int64_t)(x1[j] * g1[j]) * inv + half) >> 32) >> sh, -32768, 32767);
+        x2[j] = clamp32((int)(((int64_t)(x2[j] * g2[j]) * inv + half) >> 32) >> sh, -32768, 32767);
       }
+    }
+    // the rotated value saturates as y + 2^15 in [0, 2^16); the requantization takes the 2^15 back
+    const int64_t half = (1ll << (s.S - 1)) - ((int64_t)s.M << 15);
+    const int sh = s.S - 32;
+    int z1[8], z2[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      // of 16-bit values x1 c - x2 s stays in 32 bits with the rounding; x2 c + x1 s can be 2^31
+      const int y1 = __viaddmin_s32_relu((x1[j] * c[j] - x2[j] * n[j] + 8192) >> 14, 32768, 65535);
+      const int y2 = __viaddmin_s32_relu((int)(((int64_t)x2[j] * c[j] + (int64_t)x1[j] * n[j] + 8192) >> 14), 32768, 65535);
+      z1[j] = (int)(((int64_t)y1 * s.M + half) >> 32) >> sh;
+      z2[j] = (int)(((int64_t)y2 * s.M + half) >> 32) >> sh;
+    }
+    if (h < (is_q ? H : Hkv)) {
+      uint32_t o1[2], o2[2];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         o1[j] = pack_sat8(z1[4 * j + 1], z1[4 * j], pack_sat8(z1[4 * j + 3], z1[4 * j + 2], 0));
         o2[j] = pack_sat8(z2[4 * j + 1], z2[4 * j], pack_sat8(z2[4 * j + 3], z2[4 * j + 2], 0));
       }
-      int8_t* dst = is_q ? q8 + (int64_t)hh * D : a.k_pages + page0 + (int64_t)hh * P * D;
+      int8_t* dst = is_q ? q8 + (int64_t)h * D : a.k_pages + page0 + (int64_t)h * P * D;
       *reinterpret_cast<uint2*>(dst + sub * 8) = make_uint2(o1[0], o1[1]);
       *reinterpret_cast<uint2*>(dst + kHalf + sub * 8) = make_uint2(o2[0], o2[1]);
-    } else if (vtask < Hkv * L) {
-      *reinterpret_cast<uint4*>(a.v_pages + page0 + (int64_t)(vtask / L) * P * D + (vtask % L) * 16) = lo;
     }
     lo = next_lo;
     hi = next_hi;
@@ -247,12 +252,14 @@ __global__ void __launch_bounds__(128) k_paged_append(const llx_paged_append_arg
 
 template <int D>
 static cudaError_t launch_append_t(const llx_paged_append_args& a, const AppendSide& q, const AppendSide& k, cudaStream_t st) {
-  const int64_t parts = ((a.n_heads + 2 * a.n_kv_heads) * (D / 16) + 31) / 32;
-  // with many rows a warp takes two parts of one: the row's place is looked up once for both
-  const int64_t per_row = a.rows * parts > 148 * 64 ? (parts + 1) / 2 : parts;
+  const int64_t G = 512 / D, groups = (a.n_heads + G - 1) / G + (a.n_kv_heads + G - 1) / G + (a.n_kv_heads * D + 511) / 512;
+  // With many rows a warp takes several groups of one: the row's place is looked up and its rotation
+  // unpacked once for them.
+  int64_t per_row = groups;
+  while (per_row > 1 && a.rows * per_row > 148 * 64) per_row = (per_row + 1) / 2;
   const int64_t blocks = (a.rows * per_row + 3) / 4;
   if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
-  return launch_k(k_paged_append<D>, dim3((unsigned)blocks), dim3(128), 0, st, a, q, k, (int)parts, (int)per_row);
+  return launch_k(k_paged_append<D>, dim3((unsigned)blocks), dim3(128), 0, st, a, q, k, (int)per_row);
 }
 
 cudaError_t launch_paged_append(const llx_paged_append_args& a, cudaStream_t st) {
