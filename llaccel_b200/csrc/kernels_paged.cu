@@ -351,10 +351,12 @@ __device__ bool lists_fine(const llx_pages_args& a, const int32_t* once, const i
 
 // Releases (sign -1) or takes back (+1) every page of the listed slots; the entries stay.
 __device__ void count_pages(const llx_pages_args& a, const int32_t* slots, int sign) {
-  const int64_t total = a.n * a.max_pages;
-  for (int64_t x = threadIdx.x; x < total; x += blockDim.x) {
-    const int id = a.table[slots[x / a.max_pages] * a.table_stride + x % a.max_pages];
-    if (id >= 0 && id < a.n_pages) atomicAdd(&a.refs[id], sign);
+  for (int64_t i = threadIdx.x >> 5; i < a.n; i += blockDim.x >> 5) {
+    const int32_t* row = a.table + slots[i] * a.table_stride;
+    for (int64_t j = threadIdx.x & 31; j < a.max_pages; j += 32) {
+      const int id = row[j];
+      if (id >= 0 && id < a.n_pages) atomicAdd(&a.refs[id], sign);
+    }
   }
   __syncthreads();
 }
@@ -448,12 +450,12 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_free(const llx_pages_arg
   }
 }
 
-// children become copies of their parents; the copying itself is k_pages_fork_copy's
+// children become copies of their parents; the copying itself is k_pages_copy's
 __global__ void __launch_bounds__(kPlanThreads) k_pages_fork(const llx_pages_args a) {
   pdl_trigger();
   pdl_wait();
-  // scratch[n_pages]: whether the copying kernel has anything to do
-  int32_t* done = a.scratch + a.n_pages;
+  // scratch: the copies' targets [0, N), sources [N, 2N) and rows [2N, 3N), and [3N] their number
+  int32_t* done = a.scratch + 3 * a.n_pages;
   if (!lists_fine(a, a.list_b, a.list_a)) {
     if (threadIdx.x == 0) {
       raise_status(a.status, LLX_STATUS_BAD_SLOT);
@@ -503,8 +505,11 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_fork(const llx_pages_arg
           id = a.table[from * a.table_stride + j];
           if (id >= 0 && id < a.n_pages) atomicAdd(&a.refs[id], 1);
         } else if (j < held) {
-          id = a.scratch[base + first[x] + j - kept];
+          const int64_t m = base + first[x] + j - kept;
+          id = a.scratch[m];
           a.refs[id] = 1;
+          a.scratch[a.n_pages + m] = a.table[from * a.table_stride + j];
+          a.scratch[2 * a.n_pages + m] = (int)min(P, len - j * P);
         }
         a.table[to * a.table_stride + j] = id;
       }
@@ -513,36 +518,46 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_fork(const llx_pages_arg
     base += sum;
     __syncthreads();
   }
-  if (threadIdx.x == 0) *done = 1;
+  if (threadIdx.x == 0) *done = (int32_t)need;
 }
 
-// units of (pair, page, layer, k or v): the rows that the parent has written, head by head
-__global__ void __launch_bounds__(256) k_pages_fork_copy(const llx_pages_args a) {
+// Copies pages: block (x, y) takes moves x, x + gridDim.x, ... of layer y / 2, k or v.  `rows` null:
+// whole pages.  Four 16-byte loads per thread are under way before the first is stored; two of the
+// listed sizes (a page of 8 KB per layer) are one round.
+__global__ void __launch_bounds__(256) k_pages_copy(const llx_pages_args a, const int32_t* src, const int32_t* dst,
+                                                    const int32_t* rows, const int32_t* number) {
   pdl_trigger();
   pdl_wait();
-  if (!a.scratch[a.n_pages]) return;
-  const int64_t P = a.page_size, D = a.head_dim;
-  const int64_t units = a.n * a.max_pages * a.n_layers * 2;
-  for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
-    const int kv = (int)(u & 1);
-    int64_t x = u >> 1;
-    const int64_t layer = x % a.n_layers;
-    x /= a.n_layers;
-    const int64_t j = x % a.max_pages;
-    const int from = a.list_a[x / a.max_pages], to = a.list_b[x / a.max_pages];
-    const int64_t left = slot_length(a, from) - j * P;
-    if (left <= 0 || (a.share && left >= P)) continue;
-    const int src = a.table[from * a.table_stride + j], dst = a.table[to * a.table_stride + j];
-    if (src < 0 || src >= a.n_pages) {
-      if (threadIdx.x == 0) raise_status(a.status, LLX_STATUS_BAD_PAGE);
-      continue;
-    }
-    int8_t* pool = (kv ? a.v : a.k) + layer * a.layer_stride;
-    const int vecs = (int)((left < P ? left : P) * D / 16);
-    for (int h = 0; h < a.n_kv_heads; ++h) {
-      const uint4* s = reinterpret_cast<const uint4*>(pool + src * a.page_stride + h * P * D);
-      uint4* d = reinterpret_cast<uint4*>(pool + dst * a.page_stride + h * P * D);
-      for (int e = threadIdx.x; e < vecs; e += blockDim.x) d[e] = s[e];
+  const int moves = *number;
+  const int64_t head = a.page_size * a.head_dim;
+  const int whole = (int)(a.n_kv_heads * head / 16);
+  for (int64_t y = blockIdx.y; y < 2 * a.n_layers; y += gridDim.y) {
+    int8_t* pool = ((y & 1) ? a.v : a.k) + (y >> 1) * a.layer_stride;
+    for (int m = blockIdx.x; m < moves; m += gridDim.x) {
+      const int from = src[m], to = dst[m], held = rows ? rows[m] : (int)a.page_size;
+      if (from < 0 || from >= a.n_pages) {
+        if (threadIdx.x == 0) raise_status(a.status, LLX_STATUS_BAD_PAGE);
+        continue;
+      }
+      auto copy = [&](const int8_t* s8, int8_t* d8, int vecs) {
+        const uint4* s = reinterpret_cast<const uint4*>(s8);
+        uint4* d = reinterpret_cast<uint4*>(d8);
+        for (int e = threadIdx.x; e < vecs; e += 4 * 256) {
+          uint4 v[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (e + j * 256 < vecs) v[j] = s[e + j * 256];
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (e + j * 256 < vecs) d[e + j * 256] = v[j];
+        }
+      };
+      const int8_t* s = pool + from * a.page_stride;
+      int8_t* d = pool + to * a.page_stride;
+      if (held == a.page_size)
+        copy(s, d, whole);
+      else
+        for (int h = 0; h < a.n_kv_heads; ++h) copy(s + h * head, d + h * head, (int)(held * a.head_dim / 16));
     }
   }
 }
@@ -581,25 +596,15 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_compact(const llx_pages_
   if (threadIdx.x == 0) to[3 * N] = moves;
 }
 
-__global__ void __launch_bounds__(256) k_pages_compact_move(const llx_pages_args a) {
+// the table with the pages' new names
+__global__ void __launch_bounds__(256) k_pages_rename(const llx_pages_args a) {
   pdl_trigger();
   pdl_wait();
-  const int64_t N = a.n_pages;
-  const int32_t *to = a.scratch, *src = to + N, *dst = src + N;
   const int64_t entries = a.max_seqs * a.max_pages;
   for (int64_t x = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; x < entries; x += (int64_t)gridDim.x * blockDim.x) {
     const int64_t at = x / a.max_pages * a.table_stride + x % a.max_pages;
     const int id = a.table[at];
-    a.new_table[at] = id >= 0 && id < N ? to[id] : id;
-  }
-  const int64_t units = (int64_t)to[3 * N] * a.n_layers * 2;
-  const int vecs = (int)(a.n_kv_heads * a.page_size * a.head_dim / 16);
-  for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
-    const int64_t x = u >> 1, layer = x % a.n_layers, m = x / a.n_layers;
-    int8_t* pool = ((u & 1) ? a.v : a.k) + layer * a.layer_stride;
-    const uint4* s = reinterpret_cast<const uint4*>(pool + src[m] * a.page_stride);
-    uint4* d = reinterpret_cast<uint4*>(pool + dst[m] * a.page_stride);
-    for (int e = threadIdx.x; e < vecs; e += blockDim.x) d[e] = s[e];
+    a.new_table[at] = id >= 0 && id < a.n_pages ? a.scratch[id] : id;
   }
 }
 
@@ -616,17 +621,30 @@ cudaError_t launch_pages_free(const llx_pages_args& a, cudaStream_t st) {
   return launch_k(k_pages_free, dim3(copy_grid(blocks)), dim3(kPlanThreads), 0, st, a);
 }
 
+// enough blocks for 8 on an SM, whichever of moves and layers there are more of
+static dim3 copy_blocks(int64_t moves, int64_t layers) {
+  const int64_t y = 2 * layers < 65535 ? 2 * layers : 65535, most = (148 * 8 + y - 1) / y;
+  return dim3((unsigned)(moves < most ? (moves < 1 ? 1 : moves) : most), (unsigned)y);
+}
+
 cudaError_t launch_pages_fork(const llx_pages_args& a, cudaStream_t st) {
   if (a.n == 0) return cudaSuccess;
   const cudaError_t e = launch_k(k_pages_fork, dim3(1), dim3(kPlanThreads), 0, st, a);
   if (e != cudaSuccess) return e;
-  return launch_k(k_pages_fork_copy, dim3(copy_grid(a.n * a.max_pages * a.n_layers * 2)), dim3(256), 0, st, a);
+  const int64_t N = a.n_pages, most = a.share ? a.n : a.n * a.max_pages;
+  return launch_k(k_pages_copy, copy_blocks(most < N ? most : N, a.n_layers), dim3(256), 0, st, a,
+                  (const int32_t*)a.scratch + N, (const int32_t*)a.scratch, (const int32_t*)a.scratch + 2 * N,
+                  (const int32_t*)a.scratch + 3 * N);
 }
 
 cudaError_t launch_pages_compact(const llx_pages_args& a, cudaStream_t st) {
-  const cudaError_t e = launch_k(k_pages_compact, dim3(1), dim3(kPlanThreads), 0, st, a);
+  cudaError_t e = launch_k(k_pages_compact, dim3(1), dim3(kPlanThreads), 0, st, a);
   if (e != cudaSuccess) return e;
-  return launch_k(k_pages_compact_move, dim3(copy_grid(a.n_pages * a.n_layers * 2)), dim3(256), 0, st, a);
+  e = launch_k(k_pages_rename, dim3(copy_grid((a.max_seqs * a.max_pages + 255) / 256)), dim3(256), 0, st, a);
+  if (e != cudaSuccess) return e;
+  const int64_t N = a.n_pages;
+  return launch_k(k_pages_copy, copy_blocks(N / 2, a.n_layers), dim3(256), 0, st, a, (const int32_t*)a.scratch + N,
+                  (const int32_t*)a.scratch + 2 * N, (const int32_t*)nullptr, (const int32_t*)a.scratch + 3 * N);
 }
 
 }  // namespace llx

@@ -43,59 +43,69 @@ _ATTENTION = struct.Struct("=30q")
 _PAGES = struct.Struct("=24q")
 
 
-def _stream(device: int) -> int:
-    return torch._C._cuda_getCurrentRawStream(device)
+_I8, _I16, _I32 = torch.int8, torch.int16, torch.int32
+_stream = torch._C._cuda_getCurrentRawStream
 
 
-def _on(device, dtype, **tensors) -> None:
-    """Each tensor (None allowed) lies on `device` and has `dtype`."""
+_lib = None
+
+
+def _load():
+    global _lib
+    _lib = load_library()
+    return _lib
+
+
+def _refuse(dev: int, dtype, **tensors) -> None:
+    """Says which tensor (None allowed) is not on CUDA device `dev` or has another type.  Called when
+    a quick look over all of them found one; the quick looks keep a call's cost to a few us."""
     for name, t in tensors.items():
-        if t is None:
-            continue
-        if t.dtype is not dtype:
+        if t is not None and t.dtype is not dtype:
             raise ValueError(f"{name} must be {dtype}, not {t.dtype}")
-        if t.device != device:
-            raise ValueError(f"{name} must be on {device}, not {t.device}")
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"{name} must be on cuda:{dev}, not {t.device}")
 
 
-def _cuda(t, name: str):
-    if not t.is_cuda:
+def _cuda(t, name: str) -> int:
+    dev = t.get_device()
+    if dev < 0:
         raise ValueError(f"{name} must be a CUDA tensor: there is no CPU path")
-    return t.device
+    return dev
 
 
 def _rows(t, name: str, heads: int, dim: int, rows: int) -> int:
     """Row stride (in elements) of a [rows, heads, dim] tensor whose rows are dense."""
-    if t.dim() != 3 or t.shape[0] != rows or t.shape[1] != heads or t.shape[2] != dim:
+    if t.shape != (rows, heads, dim):
         raise ValueError(f"{name} must be [{rows}, {heads}, {dim}], not {list(t.shape)}")
     s = t.stride()
-    if rows and ((dim > 1 and s[2] != 1) or (heads > 1 and s[1] != dim)):
+    if (s[2] != 1 or s[1] != dim) and rows and ((dim > 1 and s[2] != 1) or (heads > 1 and s[1] != dim)):
         raise ValueError(f"{name}: the heads of a row must be dense")
     return s[0] if rows > 1 else heads * dim
 
 
 def _pool(k, v) -> tuple:
     """(layer stride, page stride, layers, pages, heads, page size, head dim) of k and v pages."""
-    if k.shape != v.shape or k.stride() != v.stride() or k.dim() not in (4, 5):
+    s, n = k.stride(), k.shape
+    if n != v.shape or s != v.stride() or len(n) not in (4, 5):
         raise ValueError("k_pages and v_pages must be alike: [n_pages, n_kv_heads, page_size, head_dim], "
                          "page calls also with a layer axis in front")
-    s, n = k.stride(), k.shape
     if s[-1] != 1 or s[-2] != n[-1] or s[-3] != n[-1] * n[-2]:
         raise ValueError("the heads, rows and channels of a page must be dense")
-    return (s[0] if k.dim() == 5 else 0, s[-4], n[0] if k.dim() == 5 else 1, n[-4], n[-3], n[-2], n[-1])
+    return (s[0] if len(n) == 5 else 0, s[-4], n[0] if len(n) == 5 else 1, *n[-4:])
 
 
 def _table(table, length) -> tuple:
-    if table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
+    n, s = table.shape, table.stride()
+    if len(n) != 2 or (n[1] > 1 and s[1] != 1):
         raise ValueError("table must be [slots, pages] with dense rows")
-    if length is not None and (length.dim() != 1 or length.shape[0] != table.shape[0] or
-                               (length.shape[0] > 1 and length.stride(0) != 1)):
+    if length is not None and (length.shape != (n[0],) or (n[0] > 1 and length.stride(0) != 1)):
         raise ValueError("length must be a dense vector with an entry per slot of the table")
-    return table.data_ptr(), table.stride(0) if table.shape[0] > 1 else table.shape[1], table.shape[0], table.shape[1]
+    return table.data_ptr(), s[0] if n[0] > 1 else n[1], n[0], n[1]
 
 
 def _vector(t, name: str, n: int | None = None) -> int:
-    if t.dim() != 1 or (n is not None and t.shape[0] != n) or (t.shape[0] > 1 and t.stride(0) != 1):
+    m = t.shape
+    if len(m) != 1 or (n is not None and m[0] != n) or (m[0] > 1 and t.stride(0) != 1):
         raise ValueError(f"{name} must be a dense vector" + (f" of {n} values" if n is not None else ""))
     return t.data_ptr()
 
@@ -113,6 +123,15 @@ def _need_slots(seqs, n: int, table) -> None:
         raise ValueError(f"{n} sequences, but the table has {table.shape[0]} slots")
 
 
+def _norm(x, name: str, dev: int, dim: int) -> tuple:
+    if x is None:
+        return 0, 0, 0, 0
+    gamma, eps, C, sh = x
+    if gamma.dtype is not _I16 or gamma.get_device() != dev:
+        _refuse(dev, _I16, **{name: gamma})
+    return _vector(gamma, name, dim), eps, C, sh
+
+
 def append(q, k, v, k_pages, v_pages, table, length, q_start, cos, sin, q_rq, k_rq, *, q_norm=None, k_norm=None,
            seqs=None, out=None, status=None):
     """Queries, keys and values of a launch on their way into a layer's cache.
@@ -124,38 +143,36 @@ def append(q, k, v, k_pages, v_pages, table, length, q_start, cos, sin, q_rq, k_
     to the pages of their positions.  Returns the int8 queries, in `out` if given; rows behind
     `q_start[-1]` are left as they were."""
     dev = _cuda(q, "q")
-    _on(dev, torch.int16, q=q, k=k, cos=cos, sin=sin)
-    _on(dev, torch.int8, v=v, k_pages=k_pages, v_pages=v_pages, out=out)
-    _on(dev, torch.int32, table=table, length=length, q_start=q_start, seqs=seqs, status=status)
-    if q.dim() != 3 or k_pages.dim() != 4:
+    if (not (q.dtype is k.dtype is cos.dtype is sin.dtype is _I16) or not (v.dtype is k_pages.dtype is v_pages.dtype is _I8)
+            or not (table.dtype is length.dtype is q_start.dtype is _I32)
+            or not (dev == k.get_device() == v.get_device() == k_pages.get_device() == v_pages.get_device()
+                    == table.get_device() == length.get_device() == q_start.get_device() == cos.get_device()
+                    == sin.get_device()) or out is not None or seqs is not None or status is not None):
+        _refuse(dev, _I16, q=q, k=k, cos=cos, sin=sin)
+        _refuse(dev, _I8, v=v, k_pages=k_pages, v_pages=v_pages, out=out)
+        _refuse(dev, _I32, table=table, length=length, q_start=q_start, seqs=seqs, status=status)
+    if len(q.shape) != 3 or len(k_pages.shape) != 4:
         raise ValueError("q must be [rows, n_heads, head_dim], k_pages [n_pages, n_kv_heads, page_size, head_dim]")
     R, H, D = q.shape
     _, page_stride, _, n_pages, Hkv, P, Dk = _pool(k_pages, v_pages)
     if D != Dk:
         raise ValueError(f"q has heads of {D}, the cache of {Dk}")
-    if cos.dim() != 2 or cos.shape != sin.shape or cos.shape[1] != D // 2 or not (cos.is_contiguous() and sin.is_contiguous()):
+    rot = cos.shape
+    if len(rot) != 2 or rot != sin.shape or rot[1] != D // 2 or not (cos.is_contiguous() and sin.is_contiguous()):
         raise ValueError(f"cos and sin must be dense [positions, {D // 2}]")
     if out is None:
-        out = torch.zeros((R, H, D), dtype=torch.int8, device=dev)
+        out = torch.zeros((R, H, D), dtype=_I8, device=k_pages.device)
     starts, slots, n = _launch(q_start, seqs)
     _need_slots(seqs, n, table)
-    norms = []
-    for name, x in (("q_norm", q_norm), ("k_norm", k_norm)):
-        if x is None:
-            norms.append((0, 0, 0, 0))
-            continue
-        gamma, eps, C, sh = x
-        _on(dev, torch.int16, **{name: gamma})
-        norms.append((_vector(gamma, name, D), eps, C, sh))
-    (qg, qe, qC, qsh), (kg, ke, kC, ksh) = norms
-    dev_i = dev.index
+    qg, qe, qC, qsh = _norm(q_norm, "q_norm", dev, D)
+    kg, ke, kC, ksh = _norm(k_norm, "k_norm", dev, D)
     args = _APPEND.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _rows(q, "q", H, D, R),
                         _rows(k, "k", Hkv, D, R), _rows(v, "v", Hkv, D, R), _rows(out, "out", H, D, R), R, H, Hkv, D, qg, kg,
-                        qe, qC, qsh, ke, kC, ksh, cos.data_ptr(), sin.data_ptr(), cos.shape[0], *q_rq, *k_rq,
+                        qe, qC, qsh, ke, kC, ksh, cos.data_ptr(), sin.data_ptr(), rot[0], *q_rq, *k_rq,
                         k_pages.data_ptr(), v_pages.data_ptr(), page_stride, n_pages, P, *_table(table, length),
-                        length.data_ptr(), starts, slots, n, status.data_ptr() if status is not None else 0, dev_i)
-    lib = load_library()
-    code = lib.llx_paged_append(args, _stream(dev_i))
+                        length.data_ptr(), starts, slots, n, status.data_ptr() if status is not None else 0, dev)
+    lib = _lib or _load()
+    code = lib.llx_paged_append(args, _stream(dev))
     if code:
         _check_code(lib, code)
     return out
@@ -171,25 +188,27 @@ def attention(q8, k_pages, v_pages, table, length, q_start, score_rq, out_rq, *,
     not computed.  Keys whose page id lies outside the cache count as absent; a row without keys
     gets zeros."""
     dev = _cuda(q8, "q8")
-    _on(dev, torch.int8, q8=q8, k_pages=k_pages, v_pages=v_pages, out=out)
-    _on(dev, torch.int32, table=table, length=length, q_start=q_start, seqs=seqs, status=status)
-    if q8.dim() != 3 or k_pages.dim() != 4:
+    if (not (q8.dtype is k_pages.dtype is v_pages.dtype is _I8) or not (table.dtype is length.dtype is q_start.dtype is _I32)
+            or not (dev == k_pages.get_device() == v_pages.get_device() == table.get_device() == length.get_device()
+                    == q_start.get_device()) or out is not None or seqs is not None or status is not None):
+        _refuse(dev, _I8, q8=q8, k_pages=k_pages, v_pages=v_pages, out=out)
+        _refuse(dev, _I32, table=table, length=length, q_start=q_start, seqs=seqs, status=status)
+    if len(q8.shape) != 3 or len(k_pages.shape) != 4:
         raise ValueError("q8 must be [rows, n_heads, head_dim], k_pages [n_pages, n_kv_heads, page_size, head_dim]")
     R, H, D = q8.shape
     _, page_stride, _, n_pages, Hkv, P, Dk = _pool(k_pages, v_pages)
     if D != Dk:
         raise ValueError(f"q8 has heads of {D}, the cache of {Dk}")
     if out is None:
-        out = torch.zeros((R, H, D), dtype=torch.int8, device=dev)
+        out = torch.zeros((R, H, D), dtype=_I8, device=k_pages.device)
     starts, slots, n = _launch(q_start, seqs)
     _need_slots(seqs, n, table)
-    dev_i = dev.index
     args = _ATTENTION.pack(q8.data_ptr(), out.data_ptr(), _rows(q8, "q8", H, D, R), _rows(out, "out", H, D, R), R, H, Hkv, D,
                            k_pages.data_ptr(), v_pages.data_ptr(), page_stride, n_pages, P, *_table(table, length),
                            length.data_ptr(), starts, slots, n, max_rows, max_len, *score_rq, *out_rq, prob_bits,
-                           status.data_ptr() if status is not None else 0, dev_i)
-    lib = load_library()
-    code = lib.llx_paged_attention(args, _stream(dev_i))
+                           status.data_ptr() if status is not None else 0, dev)
+    lib = _lib or _load()
+    code = lib.llx_paged_attention(args, _stream(dev))
     if code:
         _check_code(lib, code)
     return out
@@ -198,22 +217,22 @@ def attention(q8, k_pages, v_pages, table, length, q_start, score_rq, out_rq, *,
 def _page_call(name, pool, table, length, refs, list_a, list_b, share, new_table, new_refs, status) -> None:
     k, v, shape = pool
     dev = _cuda(table, "table")
-    _on(dev, torch.int32, table=table, length=length, refs=refs, list_a=list_a, list_b=list_b, new_table=new_table,
-        new_refs=new_refs, status=status)
-    _on(dev, torch.int8, k_pages=k, v_pages=v)
+    _refuse(dev, _I32, table=table, length=length, refs=refs, list_a=list_a, list_b=list_b, new_table=new_table,
+            new_refs=new_refs, status=status)
+    _refuse(dev, _I8, k_pages=k, v_pages=v)
     layer_stride, page_stride, L, n_pages, Hkv, P, D = shape
     refs_ptr = _vector(refs, "refs", n_pages)
     n = list_a.shape[0] if list_a is not None else 0
     a = _vector(list_a, "the first list") if list_a is not None else 0
     b = _vector(list_b, "the second list", n) if list_b is not None else 0
-    scratch = torch.empty(3 * n_pages + 4, dtype=torch.int32, device=dev)
+    scratch = torch.empty(3 * n_pages + 4, dtype=_I32, device=table.device)
     args = _PAGES.pack(k.data_ptr() if k is not None else 0, v.data_ptr() if v is not None else 0, layer_stride, page_stride,
                        L, n_pages, Hkv, P, D, *_table(table, length), length.data_ptr() if length is not None else 0,
                        refs_ptr, a, b, n, int(share), new_table.data_ptr() if new_table is not None else 0,
                        new_refs.data_ptr() if new_refs is not None else 0, scratch.data_ptr(),
-                       status.data_ptr() if status is not None else 0, dev.index)
-    lib = load_library()
-    code = getattr(lib, name)(args, _stream(dev.index))
+                       status.data_ptr() if status is not None else 0, dev)
+    lib = _lib or _load()
+    code = getattr(lib, name)(args, _stream(dev))
     if code:
         _check_code(lib, code)
 

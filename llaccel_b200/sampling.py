@@ -7,7 +7,7 @@ import torch
 
 from .cuda_backend import _check as _check_code
 from .cuda_backend import load_library
-from .paged import _cuda, _on, _stream, _vector
+from .paged import _cuda, _refuse, _stream, _vector
 
 _SAMPLE = struct.Struct("=13q")
 
@@ -23,28 +23,28 @@ def sample(logits, random, *, exponent, vocab=None, temperature=None, top_k=None
     is computed in integers, so the same inputs give the same tokens on any split of the work.
     Returns (tokens int32, probability float32 of each token among the kept ones), in `out` if given."""
     dev = _cuda(logits, "logits")
-    if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+    if len(logits.shape) != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise ValueError("logits must be [rows, vocabulary] with dense rows")
     R, ld = logits.shape
     V = ld if vocab is None else vocab
     if V > ld:
         raise ValueError(f"vocab {V} exceeds the {ld} columns of logits")
-    _on(dev, torch.int16, logits=logits)
-    _on(dev, torch.float32, temperature=temperature, top_p=top_p, min_p=min_p)
-    _on(dev, torch.int32, top_k=top_k)
-    _on(dev, torch.float64, random=random)
+    _refuse(dev, torch.int16, logits=logits)
+    _refuse(dev, torch.float32, temperature=temperature, top_p=top_p, min_p=min_p)
+    _refuse(dev, torch.int32, top_k=top_k)
+    _refuse(dev, torch.float64, random=random)
     ptr = [_vector(t, name, R) if t is not None else 0
            for name, t in (("temperature", temperature), ("top_p", top_p), ("min_p", min_p), ("top_k", top_k))]
     if out is None:
-        token, prob = torch.empty(R, dtype=torch.int32, device=dev), torch.empty(R, dtype=torch.float32, device=dev)
+        token, prob = torch.empty(R, dtype=torch.int32, device=logits.device), torch.empty(R, dtype=torch.float32, device=logits.device)
     else:
         token, prob = out
-        _on(dev, torch.int32, token=token)
-        _on(dev, torch.float32, prob=prob)
+        _refuse(dev, torch.int32, token=token)
+        _refuse(dev, torch.float32, prob=prob)
     args = _SAMPLE.pack(logits.data_ptr(), logits.stride(0) if R > 1 else ld, R, V, exponent, *ptr,
-                        _vector(random, "random", R), _vector(token, "token", R), _vector(prob, "prob", R), dev.index)
+                        _vector(random, "random", R), _vector(token, "token", R), _vector(prob, "prob", R), dev)
     lib = load_library()
-    code = lib.llx_sample(args, _stream(dev.index))
+    code = lib.llx_sample(args, _stream(dev))
     if code:
         _check_code(lib, code)
     return token, prob
