@@ -525,10 +525,19 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_fork(const llx_pages_arg
 // whole pages.  Four 16-byte loads per thread are under way before the first is stored; two of the
 // listed sizes (a page of 8 KB per layer) are one round.
 __global__ void __launch_bounds__(256) k_pages_copy(const llx_pages_args a, const int32_t* src, const int32_t* dst,
-                                                    const int32_t* rows, const int32_t* number) {
+                                                    const int32_t* rows, const int32_t* number,
+                                                    const int32_t* names) {
   pdl_trigger();
   pdl_wait();
   const int moves = *number;
+  if (names && blockIdx.y == 0) {  // the table with the pages' new names
+    const int64_t entries = a.max_seqs * a.max_pages;
+    for (int64_t x = blockIdx.x * 256ll + threadIdx.x; x < entries; x += gridDim.x * 256ll) {
+      const int64_t at = x / a.max_pages * a.table_stride + x % a.max_pages;
+      const int id = a.table[at];
+      a.new_table[at] = id >= 0 && id < a.n_pages ? names[id] : id;
+    }
+  }
   const int64_t head = a.page_size * a.head_dim;
   const int whole = (int)(a.n_kv_heads * head / 16);
   for (int64_t y = blockIdx.y; y < 2 * a.n_layers; y += gridDim.y) {
@@ -570,19 +579,25 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_compact(const llx_pages_
   const int64_t N = a.n_pages, per = (N + kPlanThreads - 1) / kPlanThreads;
   const int64_t p0 = min(N, threadIdx.x * per), p1 = min(N, p0 + per);
   int32_t *to = a.scratch, *src = to + N, *dst = src + N;
-  int used = 0, live, moves, holes_total;
+  int used = 0, live, moves;
   for (int64_t p = p0; p < p1; ++p) used += a.refs[p] > 0;
-  block_scan(used, &live);
-  // movers: live pages from id `live` on; holes: free pages below it; as many of each
-  int movers = 0, holes = 0;
-  for (int64_t p = p0; p < p1; ++p) {
-    movers += a.refs[p] > 0 && p >= live;
-    holes += a.refs[p] <= 0 && p < live;
+  const int before = block_scan(used, &live);  // live pages below p0
+  // movers: live pages from id `live` on; holes: free pages below it; as many of each.  Of the pages
+  // below `live`, those that are not live are holes; of the live pages, those past the ones below it move.
+  __shared__ int live_below;  // live pages with an id below `live`
+  if (p0 <= live && live < p1 + (p1 == N)) {
+    int n = before;
+    for (int64_t p = p0; p < p1 && p < live; ++p) n += a.refs[p] > 0;
+    live_below = n;
   }
-  int m = block_scan(movers, &moves), h = block_scan(holes, &holes_total);
+  __syncthreads();
+  moves = live - live_below;
+  int n = before;
   for (int64_t p = p0; p < p1; ++p) {
-    if (a.refs[p] <= 0 && p < live) dst[h++] = (int32_t)p;
-    if (a.refs[p] > 0 && p >= live) src[m++] = (int32_t)p;
+    const bool l = a.refs[p] > 0;
+    if (!l && p < live) dst[p - n] = (int32_t)p;  // free pages below p
+    if (l && p >= live) src[n - live_below] = (int32_t)p;
+    n += l;
     to[p] = (int32_t)p;
   }
   __syncthreads();
@@ -594,18 +609,6 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_compact(const llx_pages_
   __syncthreads();
   for (int64_t p = live + threadIdx.x; p < N; p += blockDim.x) a.new_refs[p] = 0;
   if (threadIdx.x == 0) to[3 * N] = moves;
-}
-
-// the table with the pages' new names
-__global__ void __launch_bounds__(256) k_pages_rename(const llx_pages_args a) {
-  pdl_trigger();
-  pdl_wait();
-  const int64_t entries = a.max_seqs * a.max_pages;
-  for (int64_t x = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; x < entries; x += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t at = x / a.max_pages * a.table_stride + x % a.max_pages;
-    const int id = a.table[at];
-    a.new_table[at] = id >= 0 && id < a.n_pages ? a.scratch[id] : id;
-  }
 }
 
 static unsigned copy_grid(int64_t units) { return (unsigned)(units < 1 ? 1 : units > 148 * 8 ? 148 * 8 : units); }
@@ -634,17 +637,15 @@ cudaError_t launch_pages_fork(const llx_pages_args& a, cudaStream_t st) {
   const int64_t N = a.n_pages, most = a.share ? a.n : a.n * a.max_pages;
   return launch_k(k_pages_copy, copy_blocks(most < N ? most : N, a.n_layers), dim3(256), 0, st, a,
                   (const int32_t*)a.scratch + N, (const int32_t*)a.scratch, (const int32_t*)a.scratch + 2 * N,
-                  (const int32_t*)a.scratch + 3 * N);
+                  (const int32_t*)a.scratch + 3 * N, (const int32_t*)nullptr);
 }
 
 cudaError_t launch_pages_compact(const llx_pages_args& a, cudaStream_t st) {
-  cudaError_t e = launch_k(k_pages_compact, dim3(1), dim3(kPlanThreads), 0, st, a);
-  if (e != cudaSuccess) return e;
-  e = launch_k(k_pages_rename, dim3(copy_grid((a.max_seqs * a.max_pages + 255) / 256)), dim3(256), 0, st, a);
+  const cudaError_t e = launch_k(k_pages_compact, dim3(1), dim3(kPlanThreads), 0, st, a);
   if (e != cudaSuccess) return e;
   const int64_t N = a.n_pages;
   return launch_k(k_pages_copy, copy_blocks(N / 2, a.n_layers), dim3(256), 0, st, a, (const int32_t*)a.scratch + N,
-                  (const int32_t*)a.scratch + 2 * N, (const int32_t*)nullptr, (const int32_t*)a.scratch + 3 * N);
+                  (const int32_t*)a.scratch + 2 * N, (const int32_t*)nullptr, (const int32_t*)a.scratch + 3 * N, (const int32_t*)a.scratch);
 }
 
 }  // namespace llx
