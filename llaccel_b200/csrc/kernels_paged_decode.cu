@@ -2,7 +2,7 @@
 //
 // A cluster of C CTAs serves one (sequence, KV head, group of up to 8 stacked (row, head) pairs);
 // each CTA takes a slice of the keys.  One thread streams the slice's K rows, then its V rows,
-// page by page through a ring of TMA-filled stages; four warps consume them, so every byte of the
+// page by page through a ring of TMA-filled stages; eight warps consume them, so every byte of the
 // cache is read once:
 //   scores  S^T (16 keys x 8 pairs) = K (16 x 32) Q^T per int8 MMA, kept in shared memory;
 //   maxima  of the slices meet in every CTA of the cluster (the reference's global maximum);
@@ -18,12 +18,13 @@
 namespace llx {
 namespace {
 
-constexpr int kConsumers = 128, kThreads = 160;  // four warps and the loading warp
+constexpr int kWarps = 8, kConsumers = kWarps * 32, kThreads = kConsumers + 32;  // and the loading warp
 constexpr int kPairs = 8;                        // stacked (row, head) pairs per CTA
-constexpr int kTK = 128;                         // keys per stage: 32 per warp
+constexpr int kTK = 128;                         // keys per stage
 constexpr int kMaxCluster = 16;
-template <int D>
-constexpr int kRing = D == 128 ? 3 : 4;  // 48 KB / 32 KB in flight per CTA
+constexpr size_t kSmemMost = 220 * 1024;         // of a CTA, its 5 KB of static arrays included
+constexpr int kMaxRing = 4;  // stages
+constexpr int kOrdered = 512;  // sequences whose order a block works out
 
 // row stride of the scores in words, = 8 mod 32: a warp's 8-byte reads of 4 pairs x 8 keys and its
 // stores hit different banks
@@ -32,23 +33,26 @@ __host__ __device__ constexpr int score_stride(int cap) { return (cap + 31) / 32
 struct DecodeShape {
   int cluster, cap, box;  // CTAs per cluster, keys per slice (multiple of 64), rows per TMA box
   int nr;                 // score rows held
+  int ring;               // stages
 };
 
 template <int D>
-__host__ __device__ inline size_t decode_smem(int nr, int cap, int P) {
-  return 1024 + (size_t)kRing<D> * kTK * D + (size_t)nr * score_stride(cap) * 4 + (size_t)2 * nr * D * 4 +
+__host__ __device__ inline size_t decode_smem(int nr, int cap, int P, int ring) {
+  return 1024 + (size_t)ring * kTK * D + (size_t)nr * score_stride(cap) * 4 + (size_t)2 * nr * D * 4 +
          (size_t)(cap / P + 2) * 4;
 }
 
 template <int D, bool HIGH>
 __global__ void __launch_bounds__(kThreads) k_paged_decode(const llx_paged_attention_args a, const __grid_constant__ CUtensorMap mk,
                                                            const __grid_constant__ CUtensorMap mv, const DecodeShape shape,
-                                                           const int most) {
-  constexpr int S = kRing<D>, KB = D / 32, MB = D / 16;
+                                                           const int most, const bool ordered) {
+  constexpr int KB = D / 32, MB = D / 16;
+  const int S = shape.ring;
   extern __shared__ unsigned char raw[];
-  __shared__ __align__(8) uint64_t full[S], empty[S], met[3];
-  __shared__ int lost, any_bad;
-  __shared__ uint32_t xmax[kMaxCluster * kPairs], xsum[kMaxCluster * kPairs], wred[4 * kPairs];
+  __shared__ __align__(8) uint64_t full[kMaxRing], empty[kMaxRing], met[3];
+  __shared__ int lost, any_bad, chosen;
+  __shared__ int lens[kOrdered];
+  __shared__ uint32_t xmax[kMaxCluster * kPairs], xsum[kMaxCluster * kPairs], wred[kWarps * kPairs], gather[kPairs];
   __shared__ uint16_t expi[18], expf[256];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int C = shape.cluster;
@@ -56,17 +60,36 @@ __global__ void __launch_bounds__(kThreads) k_paged_decode(const llx_paged_atten
   if (tid == 0) {
     for (int s = 0; s < S; ++s) {
       pa::bar_init(&full[s], 1);
-      pa::bar_init(&empty[s], kConsumers / 32);
+      pa::bar_init(&empty[s], kWarps);
     }
     for (int s = 0; s < 3; ++s) pa::bar_init(&met[s], C);
     lost = any_bad = 0;
+    for (int n = 0; n < kPairs; ++n) gather[n] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   for (int x = tid; x < 256; x += kThreads) expf[x] = kDevExpF[x];
   if (tid < 18) expi[tid] = tid < 16 ? kDevExpI[tid] : 0;
   pdl_trigger();
   pdl_wait();
-  const int i = blockIdx.x / C, kvh = blockIdx.y;
+  const int kvh = blockIdx.y;
+  int i = blockIdx.x / C;
+  // More clusters than a wave holds: the longest sequences start first, so that the last to run are
+  // short.  A block ranks the lengths itself.
+  if (ordered) {
+    const int n = (int)a.n_seqs;
+    for (int x = tid; x < n; x += kThreads) {
+      const int slot = a.seqs ? a.seqs[x] : x;
+      lens[x] = slot >= 0 && slot < a.max_seqs ? a.length[slot] : 0;
+    }
+    __syncthreads();
+    for (int x = tid; x < n; x += kThreads) {
+      int before = 0;
+      for (int y = 0; y < n; ++y) before += lens[y] > lens[x] || (lens[y] == lens[x] && y < x);
+      if (before == i) chosen = x;
+    }
+    __syncthreads();
+    i = chosen;
+  }
   const SeqView sv = view_sequence(a, i);
   const int rep = (int)(a.n_heads / a.n_kv_heads), P = (int)a.page_size;
   const int pshift = 31 - __clz(P);  // pages hold a power of two
@@ -119,12 +142,13 @@ __global__ void __launch_bounds__(kThreads) k_paged_decode(const llx_paged_atten
   }
   if (tid == 0 && any_bad) raise_status(a.status, LLX_STATUS_BAD_PAGE);
 
-  if (warp == kConsumers / 32) {
+  if (warp == kWarps) {
     if (lane == 0) {
       const int bshift = 31 - __clz(shape.box);
-      for (int it = 0; it < 2 * tiles; ++it) {
-        const int s = it % S, t0 = (it < tiles ? it : it - tiles) * kTK;
-        if (it >= S && !pa::bar_wait(&empty[s], (uint32_t)(it / S - 1) & 1, &lost)) break;
+      uint32_t turn = 1;
+      for (int it = 0, s = 0; it < 2 * tiles; ++it) {
+        const int t0 = (it < tiles ? it : it - tiles) * kTK;
+        if (it >= S && !pa::bar_wait(&empty[s], turn, &lost)) break;
         const int boxes = (min(kTK, nkeys - t0) + shape.box - 1) >> bshift;
         pa::bar_expect(&full[s], (uint32_t)(boxes * shape.box * D));
         for (int b = 0; b < boxes; ++b) {
@@ -132,6 +156,10 @@ __global__ void __launch_bounds__(kThreads) k_paged_decode(const llx_paged_atten
           // absent pages: page 0 is read in their place, its keys are never used
           pa::load_rows(ring + s * kTK * D + b * shape.box * D, it < tiles ? &mk : &mv, &full[s], kvh * P + (key & (P - 1)),
                         max(ids[(key >> pshift) - p0], 0));
+        }
+        if (++s == S) {
+          s = 0;
+          turn ^= 1;
         }
       }
     }
@@ -151,35 +179,46 @@ __global__ void __launch_bounds__(kThreads) k_paged_decode(const llx_paged_atten
     const int ra = 2 * tig, rb = ra + 1;
     const int Ta = ra < nr ? keys_of(ra) - k0 : 0, Tb = rb < nr ? keys_of(rb) - k0 : 0;  // visible keys of the slice
     int mxa = INT_MIN, mxb = INT_MIN;
-    for (int it = 0; it < tiles; ++it) {
-      const int s = it % S;
-      pa::bar_wait(&full[s], (uint32_t)(it / S) & 1, &lost);
-      const int t0 = it * kTK + warp * 32;
-      if (t0 < nkeys) {
-        const uint32_t tile = pa::s32(ring + s * kTK * D);
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          int32_t c[4] = {0, 0, 0, 0};
-#pragma unroll
-          for (int kb = 0; kb < KB; ++kb) {
-            uint32_t f[4];
-            pa::ldmatrix4(f, tile + pa::tile_at<D>(warp * 32 + m * 16 + (lane & 15), kb * 2 + (lane >> 4)));
-            pa::mma16832<false>(c, f[0], f[1], f[2], f[3], qf[kb][0], qf[kb][1]);
-          }
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int t = t0 + m * 16 + h * 8 + g;  // key of the slice
-            const bool there = !any_bad || t >= nkeys || ids[((k0 + t) >> pshift) - p0] >= 0;
-            const int va = t < Ta && there ? c[2 * h] : INT_MIN, vb = t < Tb && there ? c[2 * h + 1] : INT_MIN;
-            if (ra < nr) sc[ra * ss + t] = va;
-            if (rb < nr) sc[rb * ss + t] = vb;
-            mxa = max(mxa, va);
-            mxb = max(mxb, vb);
-          }
-        }
-      }
+    int s = 0;  // stage, and the turn of the ring
+    uint32_t turn = 0;
+    auto done = [&]() {
       __syncwarp();
       if (lane == 0) pa::bar_arrive(&empty[s]);
+      if (++s == S) {
+        s = 0;
+        turn ^= 1;
+      }
+    };
+    for (int it = 0; it < tiles; ++it) {
+      pa::bar_wait(&full[s], turn, &lost);
+      const int t0 = it * kTK + warp * 16;  // 16 keys per warp
+      if (t0 < nkeys) {
+        const uint32_t tile = pa::s32(ring + s * kTK * D);
+        int32_t c[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+          uint32_t f[4];
+          pa::ldmatrix4(f, tile + pa::tile_at<D>(warp * 16 + (lane & 15), kb * 2 + (lane >> 4)));
+          pa::mma16832<false>(c, f[0], f[1], f[2], f[3], qf[kb][0], qf[kb][1]);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int t = t0 + h * 8 + g;  // key of the slice
+          const bool there = !any_bad || t >= nkeys || ids[((k0 + t) >> pshift) - p0] >= 0;
+          const int va = t < Ta && there ? c[2 * h] : INT_MIN, vb = t < Tb && there ? c[2 * h + 1] : INT_MIN;
+          if (ra < nr) sc[ra * ss + t] = va;
+          if (rb < nr) sc[rb * ss + t] = vb;
+          mxa = max(mxa, va);
+          mxb = max(mxb, vb);
+        }
+      } else if (t0 < ((nkeys + 31) & ~31)) {  // the values are taken 32 keys at a time
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (ra < nr) sc[ra * ss + t0 + h * 8 + g] = INT_MIN;
+          if (rb < nr) sc[rb * ss + t0 + h * 8 + g] = INT_MIN;
+        }
+      }
+      done();
     }
 #pragma unroll
     for (int o = 4; o < 32; o <<= 1) {
@@ -207,48 +246,37 @@ __global__ void __launch_bounds__(kThreads) k_paged_decode(const llx_paged_atten
     {
       int v = INT_MIN;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) v = max(v, (int)wred[w * kPairs + tid % kPairs]);
+      for (int w = 0; w < kWarps; ++w) v = max(v, (int)wred[w * kPairs + tid % kPairs]);
       meet((uint32_t)v, xmax, &met[0]);
     }
     // ---- exponentials of the slice, in place; sums ----
     const int nfill = (nkeys + 31) & ~31;  // the score pass wrote up to here
     const GapScale gs = gap_scale<HIGH>(a.Ms, a.Ss);
     {
-      int mx[kPairs];
-      uint32_t sum[kPairs];
-#pragma unroll
-      for (int n = 0; n < kPairs; ++n) {
-        mx[n] = INT_MIN;
-        sum[n] = 0;
-        for (int c = 0; c < C; ++c) mx[n] = max(mx[n], (int)xmax[c * kPairs + n]);
-      }
-      for (int t = tid; t < nfill; t += kConsumers) {
-#pragma unroll
-        for (int n = 0; n < kPairs; ++n) {
-          if (n < nr) {
-            const int v = sc[n * ss + t];
-            const uint32_t e = table_exp(gap_index<HIGH>((uint32_t)mx[n] - (uint32_t)v, gs), expi, expf);
-            const uint32_t p = v == INT_MIN ? 0u : e;
-            sc[n * ss + t] = (int)p;
-            sum[n] += p;
-          }
+      // a pair's keys are dealt to kConsumers / nr threads, 4 neighbouring ones at a time
+      const int team = kConsumers / nr, n = tid / team;
+      uint32_t sum = 0;
+      if (n < nr) {
+        int mx = INT_MIN;
+        for (int c = 0; c < C; ++c) mx = max(mx, (int)xmax[c * kPairs + n]);
+        int4* row = reinterpret_cast<int4*>(sc + n * ss);
+#pragma unroll 2
+        for (int t = tid - n * team; t < nfill / 4; t += team) {
+          const int4 v = row[t];
+          auto weight = [&](int x) {
+            const uint32_t e = table_exp(gap_index<HIGH>((uint32_t)mx - (uint32_t)x, gs), expi, expf);
+            return x == INT_MIN ? 0u : e;
+          };
+          const uint32_t p0 = weight(v.x), p1 = weight(v.y), p2 = weight(v.z), p3 = weight(v.w);
+          row[t] = make_int4((int)p0, (int)p1, (int)p2, (int)p3);
+          sum += p0 + p1 + p2 + p3;
         }
-      }
-      // a slice has less than 2^16 keys of at most 65535: 32 bits hold its sum
-      pa::named_sync(1, kConsumers);  // wred is free again
-#pragma unroll
-      for (int n = 0; n < kPairs; ++n) {
-        const uint32_t v = __reduce_add_sync(0xffffffffu, sum[n]);
-        if (lane == n) wred[warp * kPairs + n] = v;
+        // a slice has less than 2^16 keys of at most 65535: 32 bits hold its sum
+        if (sum) atomicAdd(&gather[n], sum);
       }
       pa::named_sync(1, kConsumers);
     }
-    {
-      uint32_t v = 0;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) v += wred[w * kPairs + tid % kPairs];
-      meet(v, xsum, &met[1]);
-    }
+    meet(gather[tid % kPairs], xsum, &met[1]);
     // ---- values: weights of pair g, normalised as they are read ----
     uint64_t whole = 0;
     for (int c = 0; c < C; ++c) whole += xsum[c * kPairs + g];
@@ -256,20 +284,22 @@ __global__ void __launch_bounds__(kThreads) k_paged_decode(const llx_paged_atten
     const int psh = 31 - (int)a.prob_bits;
     const uint32_t prnd = 1u << (psh - 1), pmax = (1u << a.prob_bits) - 1u;
     const bool wide = a.prob_bits > 8;
-    int32_t ah[MB][4], al[MB][4];
+    // a warp takes 32 keys of a stage and half of the channels
+    constexpr int HB = MB / 2;
+    const int keys = (warp & 3) * 32, side = warp >> 2;
+    int32_t ah[HB][4], al[HB][4];
 #pragma unroll
-    for (int m = 0; m < MB; ++m)
+    for (int m = 0; m < HB; ++m)
 #pragma unroll
       for (int k = 0; k < 4; ++k) ah[m][k] = al[m][k] = 0;
     for (int it = tiles; it < 2 * tiles; ++it) {
-      const int s = it % S;
-      pa::bar_wait(&full[s], (uint32_t)(it / S) & 1, &lost);
-      const int t0 = (it - tiles) * kTK + warp * 32;
+      pa::bar_wait(&full[s], turn, &lost);
+      const int t0 = (it - tiles) * kTK + keys;
       if (t0 < nkeys) {
         const unsigned char* tile = ring + s * kTK * D;
-        // MMA key index 4 tig + e of a 16-key half stands for key 2 tig + (e & 1) + 8 (e >> 1),
-        // in the weights as in the values: the 16-byte reads of a quarter warp then hit 8 chunks
-        uint32_t w[2][MB * 2], bl[2], bh[2];
+        // MMA key index 4 tig + e of a 16-key half stands for key 2 tig + (e & 1) + 8 (e >> 1), in the
+        // weights as in the values: a thread's weights are two 8-byte reads
+        uint32_t w[2][HB * 2], bl[2], bh[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           uint32_t pn[4] = {0, 0, 0, 0};
@@ -285,40 +315,37 @@ __global__ void __launch_bounds__(kThreads) k_paged_decode(const llx_paged_atten
           const uint32_t p01 = __byte_perm(pn[0], pn[1], 0x5410), p23 = __byte_perm(pn[2], pn[3], 0x5410);
           bl[h] = __byte_perm(p01, p23, 0x6420);
           bh[h] = __byte_perm(p01, p23, 0x7531);
-          const int r0 = warp * 32 + h * 16 + 2 * tig;
+          const int r0 = keys + h * 16 + 2 * tig;
           if constexpr (D == 128) {
-            uint4 v[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              v[e] = *reinterpret_cast<const uint4*>(tile + pa::tile_at<D>(r0 + (e & 1) + 8 * (e >> 1), g));
-            pa::transpose4(v[0].x, v[1].x, v[2].x, v[3].x, w[h]);
-            pa::transpose4(v[0].y, v[1].y, v[2].y, v[3].y, w[h] + 4);
-            pa::transpose4(v[0].z, v[1].z, v[2].z, v[3].z, w[h] + 8);
-            pa::transpose4(v[0].w, v[1].w, v[2].w, v[3].w, w[h] + 12);
-          } else {
             uint2 v[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              v[e] = *reinterpret_cast<const uint2*>(tile + pa::tile_at<D>(r0 + (e & 1) + 8 * (e >> 1), g >> 1) + (g & 1) * 8);
+              v[e] = *reinterpret_cast<const uint2*>(tile + pa::tile_at<D>(r0 + (e & 1) + 8 * (e >> 1), g) + side * 8);
             pa::transpose4(v[0].x, v[1].x, v[2].x, v[3].x, w[h]);
             pa::transpose4(v[0].y, v[1].y, v[2].y, v[3].y, w[h] + 4);
+          } else {
+            uint32_t v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              v[e] = *reinterpret_cast<const uint32_t*>(tile + pa::tile_at<D>(r0 + (e & 1) + 8 * (e >> 1), g >> 1) + (g & 1) * 8 +
+                                                        side * 4);
+            pa::transpose4(v[0], v[1], v[2], v[3], w[h]);
           }
         }
 #pragma unroll
-        for (int m = 0; m < MB; ++m) {
+        for (int m = 0; m < HB; ++m) {
           pa::mma16832<true>(al[m], w[0][2 * m], w[0][2 * m + 1], w[1][2 * m], w[1][2 * m + 1], bl[0], bl[1]);
           if (wide) pa::mma16832<true>(ah[m], w[0][2 * m], w[0][2 * m + 1], w[1][2 * m], w[1][2 * m + 1], bh[0], bh[1]);
         }
       }
-      __syncwarp();
-      if (lane == 0) pa::bar_arrive(&empty[s]);
+      done();
     }
-    // block row g of m stands for channel g D / 8 + 2 m, row g + 8 for the next one
+    // block row g of m stands for channel g D / 8 + side D / 16 + 2 m, row g + 8 for the next one
 #pragma unroll
-    for (int m = 0; m < MB; ++m)
+    for (int m = 0; m < HB; ++m)
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const int n = 2 * tig + (k & 1), ch = g * (D / 8) + 2 * m + (k >> 1);
+        const int n = 2 * tig + (k & 1), ch = g * (D / 8) + side * (D / 16) + 2 * m + (k >> 1);
         if (n < nr) atomicAdd(&opart[n * D + ch], ah[m][k] * 256 + al[m][k]);
       }
     pa::named_sync(1, kConsumers);
@@ -354,14 +381,14 @@ __global__ void __launch_bounds__(kThreads) k_paged_decode(const llx_paged_atten
 }
 
 template <int D, bool HIGH>
-cudaError_t launch_decode_t(const llx_paged_attention_args& a, int most, const DecodeShape& sh, int groups, cudaStream_t st) {
+cudaError_t launch_decode_t(const llx_paged_attention_args& a, int most, const DecodeShape& sh, int groups, bool ordered, cudaStream_t st) {
   static std::atomic<bool> ready[64];
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
   if (!ready[dev].load(std::memory_order_acquire)) {
-    e = cudaFuncSetAttribute(k_paged_decode<D, HIGH>, cudaFuncAttributeMaxDynamicSharedMemorySize, 224 * 1024);
+    e = cudaFuncSetAttribute(k_paged_decode<D, HIGH>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemMost);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(k_paged_decode<D, HIGH>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return e;
     ready[dev].store(true, std::memory_order_release);
@@ -370,20 +397,18 @@ cudaError_t launch_decode_t(const llx_paged_attention_args& a, int most, const D
   e = make_page_map(&mk, a.k_pages, a, sh.box);
   if (e == cudaSuccess) e = make_page_map(&mv, a.v_pages, a, sh.box);
   if (e != cudaSuccess) return e;
-  const size_t smem = decode_smem<D>(sh.nr, sh.cap, (int)a.page_size);
+  const size_t smem = decode_smem<D>(sh.nr, sh.cap, (int)a.page_size, sh.ring);
   const dim3 grid((unsigned)(a.n_seqs * sh.cluster), (unsigned)a.n_kv_heads, (unsigned)groups);
-  if (sh.cluster == 1) return launch_k(k_paged_decode<D, HIGH>, grid, dim3(kThreads), smem, st, a, mk, mv, sh, most);
-  return launch_kc(k_paged_decode<D, HIGH>, grid, dim3(kThreads), smem, st, dim3(sh.cluster, 1, 1), a, mk, mv, sh, most);
+  if (sh.cluster == 1) return launch_k(k_paged_decode<D, HIGH>, grid, dim3(kThreads), smem, st, a, mk, mv, sh, most, ordered);
+  return launch_kc(k_paged_decode<D, HIGH>, grid, dim3(kThreads), smem, st, dim3(sh.cluster, 1, 1), a, mk, mv, sh, most, ordered);
 }
 
 int slice_cap(int64_t max_len, int C) { return (int)(((max_len + C - 1) / C + 63) / 64 * 64); }
 
-size_t smem_for(const llx_paged_attention_args& a, int nr, int64_t len, int C) {
+size_t smem_for(const llx_paged_attention_args& a, int nr, int64_t len, int C, int ring) {
   const int cap = slice_cap(len, C), P = (int)a.page_size;
-  return a.head_dim == 128 ? decode_smem<128>(nr, cap, P) : decode_smem<64>(nr, cap, P);
+  return a.head_dim == 128 ? decode_smem<128>(nr, cap, P, ring) : decode_smem<64>(nr, cap, P, ring);
 }
-
-constexpr size_t kSmemMost = 220 * 1024;
 
 int64_t longest(const llx_paged_attention_args& a) {
   const int64_t held = a.max_pages * a.page_size;
@@ -396,7 +421,7 @@ int64_t longest(const llx_paged_attention_args& a) {
 bool paged_decode_fits(const llx_paged_attention_args& a, int64_t pairs) {
   if (a.head_dim != 64 && a.head_dim != 128) return false;
   if (longest(a) > (1 << 19)) return false;  // a slice's keys and sums stay in range
-  return smem_for(a, (int)(pairs < kPairs ? pairs : kPairs), longest(a), kMaxCluster) <= kSmemMost;
+  return smem_for(a, (int)(pairs < kPairs ? pairs : kPairs), longest(a), kMaxCluster, 2) <= kSmemMost;
 }
 
 cudaError_t launch_paged_decode(const llx_paged_attention_args& a, int most, cudaStream_t st) {
@@ -407,16 +432,42 @@ cudaError_t launch_paged_decode(const llx_paged_attention_args& a, int most, cud
   sh.nr = (int)(pairs < kPairs ? pairs : kPairs);
   sh.box = a.page_size < 64 ? (int)a.page_size : 64;
   const int64_t units = a.n_seqs * a.n_kv_heads * groups;
-  // Split the keys until two CTAs per SM have work, as long as a slice keeps a stage of keys; and
-  // further where the scores would not leave room for two CTAs on an SM.
+  // Clusters that a wave holds: about 8 GPCs of 18 SMs, as many CTAs on an SM as shared memory and
+  // registers (3) allow.  A full wave streams at HBM's rate, a part-filled one at what its SMs can
+  // take (1.6 times their share); each costs the phases' latency, 5 us with one CTA on an SM, which
+  // has nothing to hide it.  The cheapest split of the keys is taken.
   int C = 1;
-  while (C < kMaxCluster && ((units * C < 2 * 148 && len > (int64_t)C * kTK) || smem_for(a, sh.nr, len, C) > 110 * 1024)) C *= 2;
-  while (C < kMaxCluster && smem_for(a, sh.nr, len, C) > kSmemMost) C *= 2;
+  double best = 1e30;
+  bool waves = false;
+  for (int c = 1; c <= kMaxCluster; c *= 2)
+    for (int ring = 2; ring <= (a.head_dim == 128 ? 3 : kMaxRing); ++ring) {
+      const size_t smem = smem_for(a, sh.nr, len, c, ring) + 5 * 1024;
+      if (smem > kSmemMost || (c > 1 && len <= (int64_t)(c / 2) * 64)) continue;
+      const int occ = (int)(227 * 1024 / smem) < 3 ? (int)(227 * 1024 / smem) : 3;
+      const int64_t wave = c == 1 ? 148 * occ : 8 * (18 * occ / c);
+      if (wave < 1) continue;
+      const double bytes = 2.0 * a.head_dim * ((len + c - 1) / c);  // of a CTA
+      const int64_t full = units / wave, rest = units % wave;
+      const double share = 6.5e3 / 148, fixed = occ == 1 ? 6000 : occ == 2 ? 3500 : 2500;
+      double t = full * (wave * c * bytes / 6.5e3 + fixed);
+      if (rest) {
+        const double even = rest * c * bytes / 6.5e3, one = bytes * ((rest * c + 147) / 148) / (1.6 * share);
+        t += (even > one ? even : one) + fixed;
+      }
+      t += (c > 1 ? 800 + 100 * c : 0) - 10 * ring;  // exchanges; the deeper ring where it costs nothing
+      if (t < best) {
+        best = t;
+        C = c;
+        sh.ring = ring;
+        waves = full > 0 && rest > 0;
+      }
+    }
+  const bool ordered = waves && a.n_seqs > 1 && a.n_seqs <= kOrdered;
   sh.cluster = C;
   sh.cap = slice_cap(len, C);
   if (a.head_dim == 128)
-    return a.Ss >= 33 ? launch_decode_t<128, true>(a, most, sh, groups, st) : launch_decode_t<128, false>(a, most, sh, groups, st);
-  return a.Ss >= 33 ? launch_decode_t<64, true>(a, most, sh, groups, st) : launch_decode_t<64, false>(a, most, sh, groups, st);
+    return a.Ss >= 33 ? launch_decode_t<128, true>(a, most, sh, groups, ordered, st) : launch_decode_t<128, false>(a, most, sh, groups, ordered, st);
+  return a.Ss >= 33 ? launch_decode_t<64, true>(a, most, sh, groups, ordered, st) : launch_decode_t<64, false>(a, most, sh, groups, ordered, st);
 }
 
 }  // namespace llx
