@@ -148,15 +148,10 @@ cudaError_t make_page_map(CUtensorMap* map, const void* base, const llx_paged_at
 cudaError_t launch_paged_attention(const llx_paged_attention_args& a, cudaStream_t st) {
   if (a.rows == 0 || a.n_seqs == 0 || a.max_rows == 0) return cudaSuccess;
   const int64_t pairs = a.max_rows * (a.n_heads / a.n_kv_heads);
+  // Up to 32 stacked pairs the cache is read once per 8 of them by the few-row kernel; from there on,
+  // and in launches that mix prompt chunks with single tokens, the chunk kernel takes every sequence.
   constexpr int kFew = 32;
-  if (paged_chunk_fits(a)) {
-    if (!paged_decode_fits(a, pairs < kFew ? pairs : kFew)) return launch_paged_chunk(a, 0, st);
-    if (pairs <= kFew) return launch_paged_decode(a, kFew, st);
-    // sequences of both kinds, unless all have the most rows
-    if (a.n_seqs * a.max_rows == a.rows) return launch_paged_chunk(a, 0, st);
-    const cudaError_t e = launch_paged_chunk(a, kFew + 1, st);
-    return e != cudaSuccess ? e : launch_paged_decode(a, kFew, st);
-  }
+  if (paged_chunk_fits(a)) return pairs <= kFew && paged_decode_fits(a, pairs) ? launch_paged_decode(a, st) : launch_paged_chunk(a, st);
   return launch_k(k_paged_attention_any, dim3((unsigned)a.rows, (unsigned)a.n_heads), dim3(256), 0, st, a);
 }
 

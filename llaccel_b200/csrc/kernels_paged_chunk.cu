@@ -10,8 +10,8 @@
 // K and V rows stream page by page through a ring filled by TMA; V is the MMA's B operand as it
 // lies (channels contiguous).  One thread owns 32 keys of one row of every tile, so maxima and sums
 // stay in registers until a pass ends.
-// Roles: warp 0 loads, warps 1 and 2 issue the MMAs (every other score tile of passes 1 and 2; the
-// scores and the values of pass 3), warps 3 to 18 do the softmax.
+// Roles: warps 0 and 1 load (every other stage), warps 2 and 3 issue the MMAs (every other score tile of
+// passes 1 and 2; the scores and the values of pass 3), warps 4 to 19 do the softmax.
 #include <atomic>
 #include <type_traits>
 
@@ -22,8 +22,12 @@ namespace llx {
 namespace {
 
 constexpr int kRows = 128, kTK = 128;
-constexpr int kSoftWarps = 16, kThreads = 96 + kSoftWarps * 32;
-constexpr int kStages = 5;
+constexpr int kSoftWarps = 16, kThreads = 128 + kSoftWarps * 32;
+// Even: the two loading warps, and in passes 1 and 2 the two issuing ones, then each keep to their own
+// stages.  A barrier's parity tells two turns apart, not three: a warp that shared a stage with the
+// other could find a turn done that has not begun.
+constexpr int kStages = 6;
+static_assert(kStages % 2 == 0, "");
 constexpr uint32_t kHidden = 0x80000000u;  // score of a key that a row does not see
 
 template <int D>
@@ -76,7 +80,7 @@ __device__ __forceinline__ void tmem_load(uint32_t addr, uint32_t (&v)[N]) {
 template <int D, bool HIGH>
 __global__ void __launch_bounds__(kThreads, 1)
     k_paged_chunk(const llx_paged_attention_args a, const __grid_constant__ CUtensorMap mk,
-                  const __grid_constant__ CUtensorMap mv, const int box, const int least, const uint32_t word) {
+                  const __grid_constant__ CUtensorMap mv, const int box, const uint32_t word) {
   using L = Smem<D>;
   constexpr uint32_t kO = 2 * kTK;  // TMEM columns: S[2], O_lo, O_hi
   extern __shared__ unsigned char raw[];
@@ -115,13 +119,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   // the last rows see the most keys: their tiles start first
   const int tile = (int)((pairs + kRows - 1) / kRows) - 1 - (int)blockIdx.x;
   const int cap = key_cap(a);
-  if (blockIdx.x == 0 && kvh == 0 && tid == 0 && pairs >= least) {
+  if (blockIdx.x == 0 && kvh == 0 && tid == 0) {
     int code = sv.code;
     if (sv.rows > a.max_rows || sv.len > cap) code |= LLX_STATUS_BAD_BOUND;
     if (!code && sv.len < sv.rows) code = LLX_STATUS_BAD_POSITION;
     if (code) raise_status(a.status, code);
   }
-  if (tile < 0 || pairs < least) return;
+  if (tile < 0) return;
   const int g0 = tile * kRows, nr = (int)min((int64_t)kRows, pairs - g0);
   auto keys_of = [&](int n) {
     const int64_t t = (int64_t)sv.len - sv.rows + (g0 + n) / rep + 1;
@@ -129,7 +133,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   };
   const int T = keys_of(nr - 1), tiles = (T + kTK - 1) / kTK;
   const int32_t* pages = a.table + (sv.slot < 0 ? 0 : sv.slot) * a.table_stride;
-  if (warp == 1) {
+  if (warp == 2) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(pa::s32(&tmem_s)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -153,9 +157,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = tmem_s;
   if (tid == 0 && any_bad) raise_status(a.status, LLX_STATUS_BAD_PAGE);
 
-  if (warp == 0) {
+  if (warp < 2) {
     // K of passes 1 and 2, then K 0, K 1, V 0, K 2, V 1, ..., V last.  A lane loads one box; the page
-    // ids of the next load are read before this one's stage is waited for.
+    // ids of the next load are read before this one's stage is waited for.  A stage costs its warp some
+    // 750 cycles of latency, hence two of them.
     const int row = lane * box;  // of the tile
     auto tile_of = [&](int it, bool* is_v) {
       const int x = it - 2 * tiles;
@@ -168,11 +173,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       return id < 0 || id >= a.n_pages ? 0 : id;  // absent: page 0 is read in its place, its keys are never used
     };
     bool is_v;
-    int t = tiles ? tile_of(0, &is_v) : 0, id = page_at(t), s = 0;
+    int t = tiles ? tile_of(warp, &is_v) : 0, id = page_at(t), s = warp;
     uint32_t turn = 1;
-    for (int it = 0; it < 4 * tiles; ++it) {
+    for (int it = warp; it < 4 * tiles; it += 2) {
       bool next_v;
-      const int next = it + 1 < 4 * tiles ? tile_of(it + 1, &next_v) : t, next_id = page_at(next);
+      const int next = it + 2 < 4 * tiles ? tile_of(it + 2, &next_v) : t, next_id = page_at(next);
       if (it >= kStages && !pa::bar_wait(&empty[s], turn, &lost)) break;
       const int boxes = (min(kTK, T - t * kTK) + box - 1) >> (31 - __clz(box));
       if (lane == 0) pa::bar_expect(&full[s], (uint32_t)(boxes * box * D));
@@ -184,12 +189,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       t = next;
       id = next_id;
       is_v = next_v;
-      if (++s == kStages) {
-        s = 0;
+      s += 2;
+      if (s >= kStages) {
+        s -= kStages;
         turn ^= 1;
       }
     }
-  } else if (warp <= 2) {
+  } else if (warp <= 3) {
     // A whole warp runs the loop and one elected thread issues: the operands' descriptors then live in
     // uniform registers.  A tile costs an issuing warp 900 cycles (two barriers, MMAs, two commits),
     // most of it latency, against 300 for the MMAs: hence two of them.
@@ -238,14 +244,32 @@ __global__ void __launch_bounds__(kThreads, 1)
       return true;
     };
     bool ok = true;
-    for (int n = warp - 1; n < 2 * tiles && ok; n += 2) ok = scores(n, n);
+    for (int n = warp - 2; n < 2 * tiles && ok; n += 2) ok = scores(n, n);
     // pass 3 loads K 0, K 1, V 0, K 2, V 1, ...
-    if (warp == 1)
+    if (warp == 2)
       for (int t = 0; t < tiles && ok; ++t) ok = scores(2 * tiles + t, 2 * tiles + (t ? 2 * t - 1 : 0));
     else
       for (int t = 0; t < tiles && ok; ++t) ok = values(t, t < tiles - 1 ? 2 * tiles + 2 * t + 2 : 4 * tiles - 1);
+  } else if ((warp & 3) * 32 >= nr) {
+    // a tile of few rows (a sequence's next token among prompt chunks): the warps past them only keep step
+    for (int st = 0; st < 3 * tiles; ++st) {
+      pa::bar_wait(&s_full[st & 1], (uint32_t)(st >> 1) & 1, &lost);
+      __syncwarp();
+      if (lane == 0) pa::bar_arrive(&s_free[st & 1]);
+      const int t = st - 2 * tiles;
+      if (t >= 0) {
+        if (t >= 2) pa::bar_wait(&p_free[t & 1], (uint32_t)((t >> 1) - 1) & 1, &lost);
+        __syncwarp();
+        if (lane == 0) pa::bar_arrive(&p_full[t & 1]);
+      }
+      if (st + 1 == tiles || st + 1 == 2 * tiles) pa::named_sync(1, kSoftWarps * 32);
+    }
+    if (tiles == 0) {
+      pa::named_sync(1, kSoftWarps * 32);
+      pa::named_sync(1, kSoftWarps * 32);
+    }
   } else {
-    const int quad = warp & 3, part = (warp - 3) >> 2;
+    const int quad = warp & 3, part = (warp - 4) >> 2;
     const int n = quad * 32 + lane;  // row of the tile
     const uint32_t lanes = (uint32_t)(quad * 32) << 16;
     const int Tn = n < nr ? keys_of(n) : 0;
@@ -388,14 +412,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   __syncthreads();
   if (lost && tid == 0) raise_status(a.status, LLX_STATUS_LOST);
-  if (warp == 1) {
+  if (warp == 2) {
     tc::tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
   }
 }
 
 template <int D, bool HIGH>
-cudaError_t launch_chunk_t(const llx_paged_attention_args& a, int64_t least, cudaStream_t st) {
+cudaError_t launch_chunk_t(const llx_paged_attention_args& a, cudaStream_t st) {
   static std::atomic<bool> ready[64];
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -413,7 +437,7 @@ cudaError_t launch_chunk_t(const llx_paged_attention_args& a, int64_t least, cud
   if (e != cudaSuccess) return e;
   const int64_t tiles = (a.max_rows * (a.n_heads / a.n_kv_heads) + kRows - 1) / kRows;
   const dim3 grid((unsigned)tiles, (unsigned)a.n_kv_heads, (unsigned)a.n_seqs);
-  return launch_k(k_paged_chunk<D, HIGH>, grid, dim3(kThreads), Smem<D>::bytes, st, a, mk, mv, box, (int)least, 4u);
+  return launch_k(k_paged_chunk<D, HIGH>, grid, dim3(kThreads), Smem<D>::bytes, st, a, mk, mv, box, 4u);
 }
 
 }  // namespace
@@ -422,11 +446,11 @@ bool paged_chunk_fits(const llx_paged_attention_args& a) {
   return (a.head_dim == 64 || a.head_dim == 128) && a.n_seqs <= 65535;
 }
 
-cudaError_t launch_paged_chunk(const llx_paged_attention_args& a, int64_t least, cudaStream_t st) {
+cudaError_t launch_paged_chunk(const llx_paged_attention_args& a, cudaStream_t st) {
   // how the quantizer normalises its multipliers; and a score of -2^31 gives an index past the table
   const bool high = a.Ss >= 33 && a.Ms < (1ll << 31) && (a.Ms >> 2 >> (a.Ss - 32)) >= 4096;
-  if (a.head_dim == 128) return high ? launch_chunk_t<128, true>(a, least, st) : launch_chunk_t<128, false>(a, least, st);
-  return high ? launch_chunk_t<64, true>(a, least, st) : launch_chunk_t<64, false>(a, least, st);
+  if (a.head_dim == 128) return high ? launch_chunk_t<128, true>(a, st) : launch_chunk_t<128, false>(a, st);
+  return high ? launch_chunk_t<64, true>(a, st) : launch_chunk_t<64, false>(a, st);
 }
 
 }  // namespace llx

@@ -12,18 +12,22 @@
 //   partial outputs are added by the CTA that finishes them, 1/C of the outputs each.
 // Integer maxima and sums: any split gives the same bits.
 #include <atomic>
+#include <mutex>
 
 #include "paged_attn.cuh"
 
 namespace llx {
 namespace {
 
-constexpr int kWarps = 8, kConsumers = kWarps * 32, kThreads = kConsumers + 32;  // and the loading warp
+constexpr int kWarps = 8, kConsumers = kWarps * 32, kLoaders = 2, kThreads = kConsumers + 32 * kLoaders;
 constexpr int kPairs = 8;                        // stacked (row, head) pairs per CTA
 constexpr int kTK = 128;                         // keys per stage
 constexpr int kMaxCluster = 16;
-constexpr size_t kSmemMost = 220 * 1024;         // of a CTA, its 5 KB of static arrays included
-constexpr int kMaxRing = 4;  // stages
+constexpr size_t kSmemMost = 220 * 1024;         // of a CTA
+constexpr size_t kStatic = 5 * 1024;             // of it, static arrays
+// dynamic shared memory with which that many CTAs fit on an SM (1 KB of each is the system's)
+constexpr size_t kSmemAt[4] = {0, kSmemMost - kStatic, 107 * 1024, 69 * 1024};
+constexpr int kMaxRing = 6;  // stages
 constexpr int kOrdered = 512;  // sequences whose order a block works out
 
 // row stride of the scores in words, = 8 mod 32: a warp's 8-byte reads of 4 pairs x 8 keys and its
@@ -38,14 +42,14 @@ struct DecodeShape {
 
 template <int D>
 __host__ __device__ inline size_t decode_smem(int nr, int cap, int P, int ring) {
-  return 1024 + (size_t)ring * kTK * D + (size_t)nr * score_stride(cap) * 4 + (size_t)2 * nr * D * 4 +
+  return 1024 + (size_t)ring * kTK * D + (size_t)nr * score_stride(cap) * 4 + (size_t)(2 * nr * D + kMaxCluster) * 4 +
          (size_t)(cap / P + 2) * 4;
 }
 
 template <int D, bool HIGH>
 __global__ void __launch_bounds__(kThreads) k_paged_decode(const llx_paged_attention_args a, const __grid_constant__ CUtensorMap mk,
                                                            const __grid_constant__ CUtensorMap mv, const DecodeShape shape,
-                                                           const int most, const bool ordered) {
+                                                           const bool ordered) {
   constexpr int KB = D / 32, MB = D / 16;
   const int S = shape.ring;
   extern __shared__ unsigned char raw[];
@@ -96,7 +100,7 @@ __global__ void __launch_bounds__(kThreads) k_paged_decode(const llx_paged_atten
   const int rows = min(sv.rows, (int)min(a.max_rows, (int64_t)INT_MAX));
   const int64_t pairs = (int64_t)rows * rep;
   const int g0 = blockIdx.z * kPairs;
-  if (pairs > most || g0 >= pairs) {  // the whole cluster agrees
+  if (g0 >= pairs) {  // the whole cluster agrees
     if (sv.code && rank == 0 && kvh == 0 && g0 == 0 && tid == 0) raise_status(a.status, sv.code);
     return;
   }
@@ -116,8 +120,8 @@ __global__ void __launch_bounds__(kThreads) k_paged_decode(const llx_paged_atten
   unsigned char* ring = base;
   int32_t* sc = reinterpret_cast<int32_t*>(base + S * kTK * D);  // [nr][ss]
   int32_t* opart = sc + shape.nr * ss;                            // [nr][D] this slice's sums
-  int32_t* xo = opart + shape.nr * D;                             // [C][nr * D / C] peers' sums of this CTA's share
-  int32_t* ids = xo + shape.nr * D;                               // page ids of the slice
+  int32_t* xo = opart + shape.nr * D;                             // [C][share] peers' sums of this CTA's share
+  int32_t* ids = xo + shape.nr * D + kMaxCluster;                               // page ids of the slice
   const int p0 = k0 >> pshift, np = nkeys ? ((k1 - 1) >> pshift) - p0 + 1 : 0;
   const int32_t* pages = a.table + (sv.slot < 0 ? 0 : sv.slot) * a.table_stride + p0;
   __syncthreads();
@@ -142,11 +146,16 @@ __global__ void __launch_bounds__(kThreads) k_paged_decode(const llx_paged_atten
   }
   if (tid == 0 && any_bad) raise_status(a.status, LLX_STATUS_BAD_PAGE);
 
-  if (warp == kWarps) {
+  if (warp >= kWarps) {
+    // A stage costs its loading warp some 750 cycles of latency (its barrier, the count of bytes, the
+    // copies), 22 bytes a cycle: two warps load every other stage.  The
+    // ring is even, so each keeps to its own stages: a barrier's parity tells two turns apart, not three,
+    // and a warp that shared a stage could find a turn done that has not begun.
     if (lane == 0) {
       const int bshift = 31 - __clz(shape.box);
+      int s = warp - kWarps;
       uint32_t turn = 1;
-      for (int it = 0, s = 0; it < 2 * tiles; ++it) {
+      for (int it = s; it < 2 * tiles; it += kLoaders) {
         const int t0 = (it < tiles ? it : it - tiles) * kTK;
         if (it >= S && !pa::bar_wait(&empty[s], turn, &lost)) break;
         const int boxes = (min(kTK, nkeys - t0) + shape.box - 1) >> bshift;
@@ -157,8 +166,9 @@ __global__ void __launch_bounds__(kThreads) k_paged_decode(const llx_paged_atten
           pa::load_rows(ring + s * kTK * D + b * shape.box * D, it < tiles ? &mk : &mv, &full[s], kvh * P + (key & (P - 1)),
                         max(ids[(key >> pshift) - p0], 0));
         }
-        if (++s == S) {
-          s = 0;
+        s += kLoaders;
+        if (s >= S) {
+          s -= S;
           turn ^= 1;
         }
       }
@@ -349,8 +359,8 @@ __global__ void __launch_bounds__(kThreads) k_paged_decode(const llx_paged_atten
         if (n < nr) atomicAdd(&opart[n * D + ch], ah[m][k] * 256 + al[m][k]);
       }
     pa::named_sync(1, kConsumers);
-    // ---- each CTA finishes 1/C of the outputs (C divides D) ----
-    const int share = nr * D / C, e0 = (int)rank * share;
+    // ---- each CTA finishes its share of the outputs ----
+    const int share = (nr * D + C - 1) / C, e0 = (int)rank * share;
     if (C > 1) {
       for (int e = tid; e < nr * D; e += kConsumers) {
         const int c = e / share;
@@ -360,7 +370,7 @@ __global__ void __launch_bounds__(kThreads) k_paged_decode(const llx_paged_atten
       if (tid < C) pa::peer_arrive(pa::peer(&met[2], (uint32_t)tid));
       pa::bar_wait<true>(&met[2], 0, &lost);
     }
-    for (int x = tid; x < share; x += kConsumers) {
+    for (int x = tid; x < share && e0 + x < nr * D; x += kConsumers) {
       int64_t o = 0;
       if (C > 1)
         for (int c = 0; c < C; ++c) o += xo[c * share + x];
@@ -380,27 +390,41 @@ __global__ void __launch_bounds__(kThreads) k_paged_decode(const llx_paged_atten
   }
 }
 
+// Clusters of each size that the device holds at once with 1, 2 or 3 CTAs on an SM, asked for once.
+struct Capacity {
+  int clusters[4][kMaxCluster + 1];
+};
 template <int D, bool HIGH>
-cudaError_t launch_decode_t(const llx_paged_attention_args& a, int most, const DecodeShape& sh, int groups, bool ordered, cudaStream_t st) {
+cudaError_t prepare_decode(int dev, const Capacity** out) {
   static std::atomic<bool> ready[64];
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return e;
+  static std::mutex lock;
+  static Capacity caps[64];
   if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
   if (!ready[dev].load(std::memory_order_acquire)) {
-    e = cudaFuncSetAttribute(k_paged_decode<D, HIGH>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemMost);
+    std::lock_guard<std::mutex> hold(lock);
+    cudaError_t e = cudaFuncSetAttribute(k_paged_decode<D, HIGH>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemMost);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(k_paged_decode<D, HIGH>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    for (int occ = 1; occ <= 3 && e == cudaSuccess; ++occ)
+      for (int c = 1; c <= kMaxCluster && e == cudaSuccess; ++c) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(c);
+        cfg.blockDim = dim3(kThreads);
+        cfg.dynamicSmemBytes = kSmemAt[occ];
+        cudaLaunchAttribute attr;
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = c;
+        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        int n = 0;
+        e = cudaOccupancyMaxActiveClusters(&n, k_paged_decode<D, HIGH>, &cfg);
+        caps[dev].clusters[occ][c] = n;
+      }
     if (e != cudaSuccess) return e;
     ready[dev].store(true, std::memory_order_release);
   }
-  CUtensorMap mk, mv;
-  e = make_page_map(&mk, a.k_pages, a, sh.box);
-  if (e == cudaSuccess) e = make_page_map(&mv, a.v_pages, a, sh.box);
-  if (e != cudaSuccess) return e;
-  const size_t smem = decode_smem<D>(sh.nr, sh.cap, (int)a.page_size, sh.ring);
-  const dim3 grid((unsigned)(a.n_seqs * sh.cluster), (unsigned)a.n_kv_heads, (unsigned)groups);
-  if (sh.cluster == 1) return launch_k(k_paged_decode<D, HIGH>, grid, dim3(kThreads), smem, st, a, mk, mv, sh, most, ordered);
-  return launch_kc(k_paged_decode<D, HIGH>, grid, dim3(kThreads), smem, st, dim3(sh.cluster, 1, 1), a, mk, mv, sh, most, ordered);
+  *out = &caps[dev];
+  return cudaSuccess;
 }
 
 int slice_cap(int64_t max_len, int C) { return (int)(((max_len + C - 1) / C + 63) / 64 * 64); }
@@ -421,53 +445,71 @@ int64_t longest(const llx_paged_attention_args& a) {
 bool paged_decode_fits(const llx_paged_attention_args& a, int64_t pairs) {
   if (a.head_dim != 64 && a.head_dim != 128) return false;
   if (longest(a) > (1 << 19)) return false;  // a slice's keys and sums stay in range
-  return smem_for(a, (int)(pairs < kPairs ? pairs : kPairs), longest(a), kMaxCluster, 2) <= kSmemMost;
+  return smem_for(a, (int)(pairs < kPairs ? pairs : kPairs), longest(a), kMaxCluster, 2) + kStatic <= kSmemMost;
 }
 
-cudaError_t launch_paged_decode(const llx_paged_attention_args& a, int most, cudaStream_t st) {
+template <int D, bool HIGH>
+static cudaError_t launch_decode_t(const llx_paged_attention_args& a, cudaStream_t st) {
+  int dev = 0;
+  const Capacity* cap = nullptr;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = prepare_decode<D, HIGH>(dev, &cap);
+  if (e != cudaSuccess) return e;
   const int64_t rep = a.n_heads / a.n_kv_heads, len = longest(a);
-  const int64_t pairs = a.max_rows * rep < most ? a.max_rows * rep : most;
+  const int64_t pairs = a.max_rows * rep;
   const int groups = (int)((pairs + kPairs - 1) / kPairs);
   DecodeShape sh;
   sh.nr = (int)(pairs < kPairs ? pairs : kPairs);
   sh.box = a.page_size < 64 ? (int)a.page_size : 64;
   const int64_t units = a.n_seqs * a.n_kv_heads * groups;
-  // Clusters that a wave holds: about 8 GPCs of 18 SMs, as many CTAs on an SM as shared memory and
-  // registers (3) allow.  A full wave streams at HBM's rate, a part-filled one at what its SMs can
-  // take (1.6 times their share); each costs the phases' latency, 5 us with one CTA on an SM, which
-  // has nothing to hide it.  The cheapest split of the keys is taken.
-  int C = 1;
+  // How many CTAs share a sequence's keys, and how deep their rings are: the cheapest by this count
+  // (bytes and ns).  A wave takes what HBM needs for its bytes (6.5 KB a ns), or what its CTAs do: a
+  // ring's bytes per 1.3 us of latency, 75 B a ns of an SM.  A wave's phases cost 6 us where a CTA is
+  // alone on its SM, less where others stream meanwhile.  Measured with 2 x 64k keys, 8 KV heads:
+  // 144 us with 16 CTAs of a sequence in two waves, 112 with two CTAs per SM, still in two.
   double best = 1e30;
   bool waves = false;
-  for (int c = 1; c <= kMaxCluster; c *= 2)
-    for (int ring = 2; ring <= (a.head_dim == 128 ? 3 : kMaxRing); ++ring) {
-      const size_t smem = smem_for(a, sh.nr, len, c, ring) + 5 * 1024;
-      if (smem > kSmemMost || (c > 1 && len <= (int64_t)(c / 2) * 64)) continue;
-      const int occ = (int)(227 * 1024 / smem) < 3 ? (int)(227 * 1024 / smem) : 3;
-      const int64_t wave = c == 1 ? 148 * occ : 8 * (18 * occ / c);
+  for (int c = 1; c <= kMaxCluster; ++c) {
+    if (c > 1 && len <= (int64_t)(c - 1) * 64) break;
+    for (int ring = 2; ring <= kMaxRing; ring += kLoaders) {  // each loading warp keeps to its own stages
+      const size_t smem = smem_for(a, sh.nr, len, c, ring) + kStatic;
+      if (smem > kSmemMost) break;
+      const int occ = smem <= kSmemAt[3] + kStatic ? 3 : smem <= kSmemAt[2] + kStatic ? 2 : 1;
+      const int64_t wave = cap->clusters[occ][c];
       if (wave < 1) continue;
-      const double bytes = 2.0 * a.head_dim * ((len + c - 1) / c);  // of a CTA
+      const double bytes = 2.0 * D * ((len + c - 1) / c);  // of a CTA
+      const double rate = ring * kTK * D / 1300.0, fixed = occ == 1 ? 6000 : occ == 2 ? 3500 : 2500;
+      auto run = [&](int64_t clusters) {  // one wave of them
+        const int64_t ctas = clusters * c, per_sm = (ctas + 147) / 148;
+        const double even = ctas * bytes / 6.5e3, own = bytes / (rate < 75.0 / per_sm ? rate : 75.0 / per_sm);
+        return (even > own ? even : own) + fixed;
+      };
       const int64_t full = units / wave, rest = units % wave;
-      const double share = 6.5e3 / 148, fixed = occ == 1 ? 6000 : occ == 2 ? 3500 : 2500;
-      double t = full * (wave * c * bytes / 6.5e3 + fixed);
-      if (rest) {
-        const double even = rest * c * bytes / 6.5e3, one = bytes * ((rest * c + 147) / 148) / (1.6 * share);
-        t += (even > one ? even : one) + fixed;
-      }
-      t += (c > 1 ? 800 + 100 * c : 0) - 10 * ring;  // exchanges; the deeper ring where it costs nothing
+      const double t = (full ? full * run(wave) : 0) + (rest ? run(rest) : 0) + (c > 1 ? 800 + 100 * c : 0);
       if (t < best) {
         best = t;
-        C = c;
+        sh.cluster = c;
         sh.ring = ring;
         waves = full > 0 && rest > 0;
       }
     }
+  }
+  if (best == 1e30) return cudaErrorInvalidConfiguration;
+  sh.cap = slice_cap(len, sh.cluster);
   const bool ordered = waves && a.n_seqs > 1 && a.n_seqs <= kOrdered;
-  sh.cluster = C;
-  sh.cap = slice_cap(len, C);
-  if (a.head_dim == 128)
-    return a.Ss >= 33 ? launch_decode_t<128, true>(a, most, sh, groups, ordered, st) : launch_decode_t<128, false>(a, most, sh, groups, ordered, st);
-  return a.Ss >= 33 ? launch_decode_t<64, true>(a, most, sh, groups, ordered, st) : launch_decode_t<64, false>(a, most, sh, groups, ordered, st);
+  CUtensorMap mk, mv;
+  e = make_page_map(&mk, a.k_pages, a, sh.box);
+  if (e == cudaSuccess) e = make_page_map(&mv, a.v_pages, a, sh.box);
+  if (e != cudaSuccess) return e;
+  const size_t smem = decode_smem<D>(sh.nr, sh.cap, (int)a.page_size, sh.ring);
+  const dim3 grid((unsigned)(a.n_seqs * sh.cluster), (unsigned)a.n_kv_heads, (unsigned)groups);
+  if (sh.cluster == 1) return launch_k(k_paged_decode<D, HIGH>, grid, dim3(kThreads), smem, st, a, mk, mv, sh, ordered);
+  return launch_kc(k_paged_decode<D, HIGH>, grid, dim3(kThreads), smem, st, dim3(sh.cluster, 1, 1), a, mk, mv, sh, ordered);
+}
+
+cudaError_t launch_paged_decode(const llx_paged_attention_args& a, cudaStream_t st) {
+  if (a.head_dim == 128) return a.Ss >= 33 ? launch_decode_t<128, true>(a, st) : launch_decode_t<128, false>(a, st);
+  return a.Ss >= 33 ? launch_decode_t<64, true>(a, st) : launch_decode_t<64, false>(a, st);
 }
 
 }  // namespace llx

@@ -211,13 +211,13 @@ __device__ __forceinline__ void transpose4(uint32_t x0, uint32_t x1, uint32_t x2
 // width; head_dim 64 or 128.
 cudaError_t make_page_map(CUtensorMap* map, const void* base, const llx_paged_attention_args& a, int box_rows);
 
-// Few query rows per sequence: at most `most` stacked (row, head) pairs per KV head; sequences
-// with more are left to the chunk kernel.  False: this geometry has no such kernel.
+// Few query rows per sequence: `pairs` stacked (row, head) pairs per KV head at most.  False: this
+// geometry has no such kernel.
 bool paged_decode_fits(const llx_paged_attention_args& a, int64_t pairs);
-cudaError_t launch_paged_decode(const llx_paged_attention_args& a, int most, cudaStream_t st);
+cudaError_t launch_paged_decode(const llx_paged_attention_args& a, cudaStream_t st);
 
-// Sequences with at least `least` stacked (row, head) pairs per KV head, any length.
+// Any number of rows and keys, head_dim 64 or 128.
 bool paged_chunk_fits(const llx_paged_attention_args& a);
-cudaError_t launch_paged_chunk(const llx_paged_attention_args& a, int64_t least, cudaStream_t st);
+cudaError_t launch_paged_chunk(const llx_paged_attention_args& a, cudaStream_t st);
 
 }  // namespace llx
