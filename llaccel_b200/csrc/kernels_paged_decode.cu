@@ -464,9 +464,10 @@ static cudaError_t launch_decode_t(const llx_paged_attention_args& a, cudaStream
   const int64_t units = a.n_seqs * a.n_kv_heads * groups;
   // How many CTAs share a sequence's keys, and how deep their rings are: the cheapest by this count
   // (bytes and ns).  A wave takes what HBM needs for its bytes (6.5 KB a ns), or what its CTAs do: a
-  // ring's bytes per 1.3 us of latency, 75 B a ns of an SM.  A wave's phases cost 6 us where a CTA is
-  // alone on its SM, less where others stream meanwhile.  Measured with 2 x 64k keys, 8 KV heads:
-  // 144 us with 16 CTAs of a sequence in two waves, 112 with two CTAs per SM, still in two.
+  // ring's bytes per 1.9 us of loaded latency, 49 B a ns of an SM with one CTA on it, 60 with more.  A wave's phases cost 6 us where a CTA is
+  // alone on its SM, less where others stream meanwhile.  Measured: 64 sequences of 1500 to 4200 keys,
+  // 8 KV heads: one CTA each, ring of 4 82 us, of 2 106; two CTAs, ring of 4 95, of 2 112.  Two of 64k
+  // keys: 10 CTAs, ring of 6 103 us; 9, 6 113; 16, 2 118; 8, 4 127.
   double best = 1e30;
   bool waves = false;
   for (int c = 1; c <= kMaxCluster; ++c) {
@@ -478,10 +479,11 @@ static cudaError_t launch_decode_t(const llx_paged_attention_args& a, cudaStream
       const int64_t wave = cap->clusters[occ][c];
       if (wave < 1) continue;
       const double bytes = 2.0 * D * ((len + c - 1) / c);  // of a CTA
-      const double rate = ring * kTK * D / 1300.0, fixed = occ == 1 ? 6000 : occ == 2 ? 3500 : 2500;
+      const double rate = ring * kTK * D / 1900.0, fixed = occ == 1 ? 6000 : occ == 2 ? 3500 : 2500;
       auto run = [&](int64_t clusters) {  // one wave of them
         const int64_t ctas = clusters * c, per_sm = (ctas + 147) / 148;
-        const double even = ctas * bytes / 6.5e3, own = bytes / (rate < 75.0 / per_sm ? rate : 75.0 / per_sm);
+        const double even = ctas * bytes / 6.5e3, most = per_sm > 1 ? 60.0 / per_sm : 49.0;
+        const double own = bytes / (rate < most ? rate : most);
         return (even > own ? even : own) + fixed;
       };
       const int64_t full = units / wave, rest = units % wave;
