@@ -300,6 +300,37 @@ typedef struct {
 } llx_sample_args;
 llx_status llx_sample(const llx_sample_args* a, void* stream);
 
+/* ---- Serving a model: sequences of different lengths over a paged cache -----------------------
+ * A step takes tokens of several sequences at once, from one each (decode) to whole prompts, runs the
+ * model's graph over their rows and returns one next token per sequence.  It is the calls above in the
+ * model's own path: pages are reserved, every layer appends to them and attends over them, the last
+ * rows are sampled.  Results are those of llx_generate on each sequence alone, bit for bit.
+ * max_seqs slots share n_pages pages of page_size positions; a step has max_rows tokens at most.
+ * One GPU, graphs of the fused op list (llx_opts.fuse = 1).  Not thread-safe; every call waits for
+ * its work. */
+typedef struct llx_serve llx_serve;
+/* per sequence of a step (each array may be null, see llx_sample); random null: largest logit */
+typedef struct {
+  const double* random;
+  const float* temperature;
+  const int32_t* top_k;
+  const float* top_p;
+  const float* min_p;
+} llx_sampling;
+llx_status llx_serve_create(llx_model* m, int max_seqs, int n_pages, int page_size, int max_rows, llx_serve** out);
+void llx_serve_destroy(llx_serve* s);
+/* counts[i] >= 1 tokens for the sequence in slots[i], the sequences' tokens one after the other (an
+ * empty slot starts a sequence); next [n], prob [n] (may be null; sampled steps only), logits [n][vocab_padded]
+ * (may be null).  LLX_ERR_OOM: too few free pages, nothing was changed. */
+llx_status llx_serve_step(llx_serve* s, int n, const int32_t* slots, const int32_t* counts, const int32_t* tokens,
+                          const llx_sampling* how, int32_t* next, float* prob, int16_t* logits);
+/* children[i] becomes a copy of parents[i] (llx_pages_fork); slots given back; live pages moved to the
+ * front; lengths [max_seqs] and the number of pages in use */
+llx_status llx_serve_fork(llx_serve* s, int n, const int32_t* parents, const int32_t* children, int share);
+llx_status llx_serve_free(llx_serve* s, int n, const int32_t* slots);
+llx_status llx_serve_compact(llx_serve* s);
+llx_status llx_serve_usage(llx_serve* s, int32_t* lengths, int* used_pages);
+
 #ifdef __cplusplus
 }
 #endif

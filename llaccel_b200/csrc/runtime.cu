@@ -34,6 +34,7 @@
 #include "launch.cuh"
 #include "luts_data.h"
 #include "numerics.cuh"
+#include "paged.h"
 
 namespace llx {
 
@@ -843,6 +844,29 @@ static void load_model(llx_model* m, const std::string& dir) {
 // ---------------------------------------------------------------------------------------
 // Session
 // ---------------------------------------------------------------------------------------
+namespace llx {
+// The cache of a paged session: one pool of pages per layer, one table for all of them, and the
+// launch under way.  A step of the plan that rotates q and k becomes one append call (with the
+// per-head norms before it, when nothing else reads their outputs), the attention reads the pages.
+struct PagedState {
+  int max_seqs = 0, n_pages = 0, page_size = 0, max_pages = 0, Hkv = 0, D = 0;
+  std::map<int, int> layer_index;  // qgraph layer -> pool
+  int8_t *k = nullptr, *v = nullptr;
+  int64_t layer_stride = 0;  // bytes between a layer's pages and the next one's, in k and in v
+  // device: table, lengths, counts, status, scratch; the launch's row starts, slots and new rows; lists
+  int32_t *table = nullptr, *length = nullptr, *refs = nullptr, *status = nullptr, *scratch = nullptr;
+  int32_t *starts = nullptr, *slots = nullptr, *counts = nullptr;
+  float *temperature = nullptr, *top_p = nullptr, *min_p = nullptr, *prob = nullptr;
+  int32_t* top_k = nullptr;
+  double* random = nullptr;
+  std::vector<void*> owned;
+  std::vector<int> len;             // host copy of the lengths
+  std::vector<int> q_norm, k_norm;  // per plan step: the norm steps its append takes over, or -1
+  std::vector<char> skipped;        // per plan step: a norm that an append takes over
+  int n = 0, rows = 0, max_rows = 0, max_len = 0;  // the launch under way
+};
+}  // namespace llx
+
 struct llx_session {
   llx_model* m = nullptr;
   int B = 0, max_rows = 0;
@@ -889,6 +913,12 @@ struct llx_session {
   bool last_tail = false;
   bool last_logits = true;  // the last launch stored its logits rows
   uint8_t* d_flush = nullptr;  // profiling: a buffer twice the L2 size, written between timed launches
+  llx::PagedState* paged = nullptr;  // a paged session's cache; its launches are ragged rows of many sequences
+};
+
+// a paged session (include/llx.h): a session of its own kind, so that the dense calls cannot be made on it
+struct llx_serve {
+  llx_session s;
 };
 
 namespace llx {
@@ -973,6 +1003,92 @@ static bool norm_folds_into_next(const llx_session* s, size_t i, int R) {
 }
 
 static int enqueue_one(llx_session* s, const Binding& bd, const Step& x, int R, int M);
+
+// The launch's queries, keys and values into the pages of the layer (plan step idx).
+static cudaError_t enqueue_paged_append(llx_session* s, const Binding& bd, const Step& x, size_t idx) {
+  const llx_model* m = s->m;
+  const PagedState& p = *s->paged;
+  const Step& q = x.parts[0];
+  const Step& k = x.parts[1];
+  const Step& v = x.parts[2];
+  llx_paged_append_args a{};
+  const int layer = p.layer_index.at(k.layer);
+  auto side = [&](int norm, const Step& rope, const int16_t** src, const int16_t** gamma, int64_t* eps, int64_t* C, int64_t* sh) {
+    *src = (const int16_t*)bd.p[rope.in];
+    if (norm < 0) return;
+    const Step& n = m->steps[norm];
+    *src = (const int16_t*)bd.p[n.in];
+    *gamma = (const int16_t*)(m->d_blob + n.gamma_off);
+    *eps = n.eps_t;
+    *C = n.C;
+    *sh = n.sh_post;
+  };
+  side(p.q_norm[idx], q, &a.q, &a.q_gamma, &a.q_eps, &a.q_C, &a.q_shift);
+  side(p.k_norm[idx], k, &a.k, &a.k_gamma, &a.k_eps, &a.k_C, &a.k_shift);
+  a.v = (const int8_t*)bd.p[v.in2];
+  a.q8 = (int8_t*)bd.p[q.out2];
+  a.q_stride = a.q8_stride = (int64_t)q.H * q.D;
+  a.k_stride = a.v_stride = (int64_t)k.H * k.D;
+  a.rows = p.rows;
+  a.n_heads = q.H;
+  a.n_kv_heads = k.H;
+  a.head_dim = q.D;
+  a.cos = (const int16_t*)(m->d_blob + m->cos_off);
+  a.sin = (const int16_t*)(m->d_blob + m->sin_off);
+  a.n_positions = m->max_seq;
+  a.q_M = q.Mq;
+  a.q_S = q.Sq;
+  a.k_M = k.Mq;
+  a.k_S = k.Sq;
+  a.k_pages = p.k + layer * p.layer_stride;
+  a.v_pages = p.v + layer * p.layer_stride;
+  a.page_stride = (int64_t)p.Hkv * p.page_size * p.D;
+  a.n_pages = p.n_pages;
+  a.page_size = p.page_size;
+  a.table = p.table;
+  a.table_stride = a.max_pages = p.max_pages;
+  a.max_seqs = p.max_seqs;
+  a.length = p.length;
+  a.q_start = p.starts;
+  a.seqs = p.slots;
+  a.n_seqs = p.n;
+  a.status = p.status;
+  return launch_paged_append(a, s->st);
+}
+
+static cudaError_t enqueue_paged_attention(llx_session* s, const Step& x, const int8_t* q8, int8_t* out) {
+  const PagedState& p = *s->paged;
+  const int layer = p.layer_index.at(x.layer);
+  llx_paged_attention_args a{};
+  a.q8 = q8;
+  a.out = out;
+  a.q8_stride = a.out_stride = (int64_t)x.H * x.D;
+  a.rows = p.rows;
+  a.n_heads = x.H;
+  a.n_kv_heads = x.Hkv;
+  a.head_dim = x.D;
+  a.k_pages = p.k + layer * p.layer_stride;
+  a.v_pages = p.v + layer * p.layer_stride;
+  a.page_stride = (int64_t)p.Hkv * p.page_size * p.D;
+  a.n_pages = p.n_pages;
+  a.page_size = p.page_size;
+  a.table = p.table;
+  a.table_stride = a.max_pages = p.max_pages;
+  a.max_seqs = p.max_seqs;
+  a.length = p.length;
+  a.q_start = p.starts;
+  a.seqs = p.slots;
+  a.n_seqs = p.n;
+  a.max_rows = p.max_rows;
+  a.max_len = p.max_len;
+  a.Ms = x.Ms;
+  a.Ss = x.Ss;
+  a.Mo = x.Mo;
+  a.So = x.So;
+  a.prob_bits = x.prob_bits;
+  a.status = p.status;
+  return launch_paged_attention(a, s->st);
+}
 
 // One tensor-core GEMM over R rows of activation `in` (N x K weights at a.W).  Many output
 // tiles (at least two per SM: prefill, the vocabulary projection) go to the persistent
@@ -1078,6 +1194,7 @@ static int enqueue_one(llx_session* s, const Binding& bd, const Step& x, int R, 
   const bool top = &x >= steps0 && &x < steps0 + m->steps.size();
   const size_t idx = top ? (size_t)(&x - steps0) : 0;
   if (top && norm_folds_into_next(s, idx, R)) return 0;
+  if (top && s->paged && s->paged->skipped[idx]) return 0;
   const Step* fold = top && idx > 0 && norm_folds_into_next(s, idx - 1, R) ? &m->steps[idx - 1] : nullptr;
   auto P = [&](int a) { return a < 0 ? nullptr : bd.p[a]; };
   // the folded RMSNorm's row and parameters for the GEMV prologue
@@ -1197,6 +1314,10 @@ static int enqueue_one(llx_session* s, const Binding& bd, const Step& x, int R, 
         break;
       }
       case SK::Attention: {
+        if (s->paged) {
+          e = enqueue_paged_attention(s, x, (const int8_t*)P(x.in), (int8_t*)P(x.out));
+          break;
+        }
         auto kv = s->kv_layer.at(x.layer);
         AttnArgs a{};
         a.q = (const int8_t*)P(x.in);
@@ -1286,6 +1407,10 @@ static int enqueue_one(llx_session* s, const Binding& bd, const Step& x, int R, 
         break;
       }
       case SK::RopeGroup: {
+        if (s->paged) {
+          e = enqueue_paged_append(s, bd, x, idx);
+          break;
+        }
         if (M == 1 && x.folded && !s->keep) return 0;  // done by the decode attention
         const Step& q = x.parts[0];
         const Step& k = x.parts[1];
@@ -1394,6 +1519,11 @@ static void plan_arena(llx_session* s) {
       if (x.kind != SK::Attention || x.rope_step < 0) continue;
       for (int a : step_ins(m->steps[x.rope_step])) last[a] = std::max(last[a], i);
     }
+    // a norm that a paged append takes over is not run: its input lives through that step
+    if (s->paged)
+      for (int i = 0; i < ns; ++i)
+        for (int nm : {s->paged->q_norm[i], s->paged->k_norm[i]})
+          if (nm >= 0) last[m->steps[nm].in] = std::max(last[m->steps[nm].in], i);
     // a norm folded into the next GEMV's prologue is read by that GEMV: its input lives
     // through it, so the GEMV's output never takes the row other blocks are still reading
     for (int i = 0; i + 1 < ns; ++i)
@@ -1597,13 +1727,14 @@ static cudaGraphExec_t build_decode_graph(llx_session* s, bool with_logits) {
 }
 
 static void session_create(llx_model* m, int batch, int max_rows, int keep, llx_session* s) {
+  const bool paged = s->paged != nullptr;
   require(batch >= 1, LLX_ERR_INVALID, "batch must be >= 1");
   if (m->tp_world > 1) {
     require(m->tp != nullptr, LLX_ERR_INVALID, "tensor-parallel rank graph: call llx_tp_init before creating a session");
     // collectives of two sessions on one communicator could interleave differently per rank
     require(m->n_sessions == 0, LLX_ERR_UNSUPPORTED, "a tensor-parallel model serves one session at a time");
   }
-  require(max_rows >= 1 && max_rows <= m->max_seq, LLX_ERR_INVALID, "max_rows must be in [1, max_seq]");
+  require(max_rows >= 1 && (paged || max_rows <= m->max_seq), LLX_ERR_INVALID, "max_rows must be in [1, max_seq]");
   s->m = m;
   m->n_sessions++;
   s->B = batch;
@@ -1612,18 +1743,21 @@ static void session_create(llx_model* m, int batch, int max_rows, int keep, llx_
   // the row-independent tail (final norm, lm_head, ...) holds every row of a launch when
   // that costs at most 2 GB of logits, else 64 recorded rows per sequence
   s->max_tail_rows = (double)batch * max_rows * m->vocab_padded * 2.0 <= 2.0e9 ? max_rows : std::min(max_rows, 64);
+  if (paged) s->max_tail_rows = std::min(max_rows, s->paged->max_seqs);  // the last row of each sequence
   LLX_CUDA(cudaSetDevice(m->device));
   LLX_CUDA(cudaStreamCreateWithFlags(&s->st, cudaStreamNonBlocking));
   plan_arena(s);
   LLX_CUDA(cudaMalloc(&s->arena, s->arena_bytes));
   LLX_CUDA(cudaMemset(s->arena, 0, s->arena_bytes));
   size_t kvb = 0;
-  for (auto& kv : m->kv_layers) kvb += 2 * (size_t)batch * kv.second.Hkv * m->max_seq * kv.second.D;
+  if (!paged)
+    for (auto& kv : m->kv_layers) kvb += 2 * (size_t)batch * kv.second.Hkv * m->max_seq * kv.second.D;
   s->kv_bytes = std::max<size_t>(kvb, 256);
   LLX_CUDA(cudaMalloc(&s->kv, s->kv_bytes));
   LLX_CUDA(cudaMemset(s->kv, 0, s->kv_bytes));
   size_t off = 0;
   for (auto& kv : m->kv_layers) {
+    if (paged) break;
     const size_t one = (size_t)batch * kv.second.Hkv * m->max_seq * kv.second.D;
     s->kv_layer[kv.first] = {s->kv + off, s->kv + off + one};
     off += 2 * one;
@@ -1659,6 +1793,9 @@ static void session_free(llx_session* s) {
     s->m->n_sessions--;
   }
   if (s->st) cudaStreamSynchronize(s->st);
+  if (s->paged)
+    for (void* p : s->paged->owned) cudaFree(p);
+  delete s->paged;
   for (cudaGraphExec_t g : s->decode_exec)
     if (g) cudaGraphExecDestroy(g);
   for (void* p : {(void*)s->arena, (void*)s->kv, (void*)s->d_tokens, (void*)s->d_rec, (void*)s->d_argmax,
@@ -1672,6 +1809,150 @@ static void session_free(llx_session* s) {
 static void reset_kv(llx_session* s) {
   LLX_CUDA(cudaMemsetAsync(s->kv, 0, s->kv_bytes, s->st));
   LLX_CUDA(cudaStreamSynchronize(s->st));
+}
+
+// ---- paged sessions -----------------------------------------------------------------------
+template <class T>
+static T* paged_alloc(PagedState& p, size_t n) {
+  void* d = nullptr;
+  LLX_CUDA(cudaMalloc(&d, std::max<size_t>(n * sizeof(T), 256)));
+  p.owned.push_back(d);
+  LLX_CUDA(cudaMemset(d, 0, n * sizeof(T)));
+  return (T*)d;
+}
+
+static void paged_create(llx_model* m, int max_seqs, int n_pages, int page_size, int max_rows, llx_session* s) {
+  require(m->tp_world == 1, LLX_ERR_UNSUPPORTED, "paged sessions serve one GPU");
+  require(max_seqs >= 1 && max_seqs <= (1 << 18), LLX_ERR_INVALID, "max_seqs must be 1 to 262144");
+  require(page_size >= 16 && page_size <= 256 && (page_size & (page_size - 1)) == 0, LLX_ERR_INVALID,
+          "page_size must be a power of two of 16 to 256");
+  require(n_pages >= 1, LLX_ERR_INVALID, "n_pages must be at least 1");
+  require(max_rows >= 1 && max_rows <= (1 << 20), LLX_ERR_INVALID, "max_rows must be 1 to 2^20");
+  s->paged = new PagedState;
+  PagedState& p = *s->paged;
+  p.max_seqs = max_seqs;
+  p.n_pages = n_pages;
+  p.page_size = page_size;
+  p.max_pages = (m->max_seq + page_size - 1) / page_size;
+  require(!m->kv_layers.empty(), LLX_ERR_UNSUPPORTED, "the graph has no attention");
+  for (auto& kv : m->kv_layers) {
+    const int at = (int)p.layer_index.size();
+    p.layer_index[kv.first] = at;
+    if (at == 0) {
+      p.Hkv = kv.second.Hkv;
+      p.D = kv.second.D;
+    }
+    require(kv.second.Hkv == p.Hkv && kv.second.D == p.D, LLX_ERR_UNSUPPORTED, "a paged cache needs layers of one KV geometry");
+  }
+  require(p.D <= 256, LLX_ERR_UNSUPPORTED, "a paged cache needs head_dim up to 256");
+  // every attention fed by a rotation group: graphs of the fused op list, loaded with fuse = 1
+  const size_t ns = m->steps.size();
+  p.q_norm.assign(ns, -1);
+  p.k_norm.assign(ns, -1);
+  p.skipped.assign(ns, 0);
+  for (size_t i = 0; i < ns; ++i) {
+    const Step& x = m->steps[i];
+    const bool ok = x.kind != SK::Rope && x.kind != SK::KvWrite &&
+                    (x.kind != SK::RopeGroup || (x.parts[2].in2 >= 0 && m->act_uses[x.parts[0].out] == 0 &&
+                                                 m->act_uses[x.parts[1].out] == 0 &&
+                                                 (x.parts[1].out2 < 0 || m->act_uses[x.parts[1].out2] == 0)));
+    require(ok, LLX_ERR_UNSUPPORTED, "a paged session needs the fused op list (step '" + x.label + "' writes a dense cache)");
+    if (x.kind != SK::RopeGroup) continue;
+    for (int side = 0; side < 2; ++side) {  // a per-head norm that feeds the rotation and nothing else
+      const Step& r = x.parts[side];
+      for (size_t j = 0; j < i; ++j) {
+        const Step& n = m->steps[j];
+        if (n.kind == SK::RmsNorm && n.out == r.in && n.out2 < 0 && n.heads == r.H && n.K == r.D && m->act_uses[n.out] == 1) {
+          (side ? p.k_norm : p.q_norm)[i] = (int)j;
+          p.skipped[j] = 1;
+        }
+      }
+    }
+  }
+  session_create(m, 1, max_rows, 0, s);
+  const size_t L = p.layer_index.size(), page = (size_t)p.Hkv * page_size * p.D;
+  p.layer_stride = (int64_t)(page * n_pages);
+  p.k = paged_alloc<int8_t>(p, L * page * n_pages);
+  p.v = paged_alloc<int8_t>(p, L * page * n_pages);
+  p.table = paged_alloc<int32_t>(p, (size_t)max_seqs * p.max_pages);
+  LLX_CUDA(cudaMemset(p.table, 0xff, sizeof(int32_t) * max_seqs * p.max_pages));
+  p.length = paged_alloc<int32_t>(p, max_seqs);
+  p.refs = paged_alloc<int32_t>(p, n_pages);
+  p.status = paged_alloc<int32_t>(p, 1);
+  p.scratch = paged_alloc<int32_t>(p, llx_pages_scratch(n_pages) / sizeof(int32_t));
+  p.starts = paged_alloc<int32_t>(p, max_seqs + 1);
+  p.slots = paged_alloc<int32_t>(p, max_seqs);
+  p.counts = paged_alloc<int32_t>(p, max_seqs);
+  p.temperature = paged_alloc<float>(p, max_seqs);
+  p.top_p = paged_alloc<float>(p, max_seqs);
+  p.min_p = paged_alloc<float>(p, max_seqs);
+  p.prob = paged_alloc<float>(p, max_seqs);
+  p.top_k = paged_alloc<int32_t>(p, max_seqs);
+  p.random = paged_alloc<double>(p, max_seqs);
+  p.len.assign(max_seqs, 0);
+  LLX_CUDA(cudaDeviceSynchronize());
+}
+
+template <class T>
+static void paged_put(llx_session* s, T* dst, const T* src, size_t n) {
+  if (n) LLX_CUDA(cudaMemcpyAsync(dst, src, n * sizeof(T), cudaMemcpyHostToDevice, s->st));
+}
+
+static llx_pages_args paged_pages(llx_session* s, int n) {
+  PagedState& p = *s->paged;
+  llx_pages_args a{};
+  a.k = p.k;
+  a.v = p.v;
+  a.layer_stride = p.layer_stride;
+  a.page_stride = (int64_t)p.Hkv * p.page_size * p.D;
+  a.n_layers = (int64_t)p.layer_index.size();
+  a.n_pages = p.n_pages;
+  a.n_kv_heads = p.Hkv;
+  a.page_size = p.page_size;
+  a.head_dim = p.D;
+  a.table = p.table;
+  a.table_stride = a.max_pages = p.max_pages;
+  a.max_seqs = p.max_seqs;
+  a.length = p.length;
+  a.refs = p.refs;
+  a.list_a = p.slots;
+  a.list_b = p.counts;
+  a.n = n;
+  a.scratch = p.scratch;
+  a.status = p.status;
+  return a;
+}
+
+// waits for the stream; what the device found wrong since the last call becomes an error
+static void paged_check(llx_session* s) {
+  PagedState& p = *s->paged;
+  int32_t code = 0;
+  LLX_CUDA(cudaMemcpyAsync(&code, p.status, sizeof(code), cudaMemcpyDeviceToHost, s->st));
+  LLX_CUDA(cudaStreamSynchronize(s->st));
+  if (!code) return;
+  LLX_CUDA(cudaMemsetAsync(p.status, 0, sizeof(code), s->st));
+  require(!(code & LLX_STATUS_NO_PAGES), LLX_ERR_OOM, "the cache has too few free pages");
+  throw Error(LLX_ERR_DEVICE, "a paged call found its tables damaged (status " + std::to_string(code) + ")");
+}
+
+static int paged_need(const PagedState& p, int len) { return (len + p.page_size - 1) / p.page_size; }
+
+// pages that are free whatever is shared: every slot counted as if it held its pages alone
+static int64_t paged_free_at_least(const PagedState& p) {
+  int64_t n = p.n_pages;
+  for (int len : p.len) n -= paged_need(p, len);
+  return n;
+}
+
+static void paged_slots(const PagedState& p, int n, const int32_t* slots, bool once) {
+  require(n >= 0 && n <= p.max_seqs && (n == 0 || slots), LLX_ERR_INVALID, "a list of at most max_seqs slots");
+  std::vector<char> seen(once ? p.max_seqs : 0, 0);
+  for (int i = 0; i < n; ++i) {
+    require(slots[i] >= 0 && slots[i] < p.max_seqs, LLX_ERR_RANGE, "slot " + std::to_string(slots[i]) + " outside [0, max_seqs)");
+    if (!once) continue;
+    require(!seen[slots[i]], LLX_ERR_INVALID, "slot " + std::to_string(slots[i]) + " is listed twice");
+    seen[slots[i]] = 1;
+  }
 }
 
 }  // namespace llx
@@ -2182,6 +2463,184 @@ llx_status llx_read_activation(llx_session* s, const char* name, void* dst, size
     LLX_CUDA(cudaStreamSynchronize(s->st));
     LLX_CUDA(cudaMemcpy(dst, s->arena + s->act_off[a], need, cudaMemcpyDeviceToHost));
     if (rows_out) *rows_out = rows;
+  });
+}
+
+llx_status llx_serve_create(llx_model* m, int max_seqs, int n_pages, int page_size, int max_rows, llx_serve** out) {
+  return guarded([&] {
+    require(m && out, LLX_ERR_INVALID, "null argument");
+    auto h = std::make_unique<llx_serve>();
+    try {
+      paged_create(m, max_seqs, n_pages, page_size, max_rows, &h->s);
+    } catch (...) {
+      session_free(&h->s);
+      throw;
+    }
+    *out = h.release();
+  });
+}
+
+void llx_serve_destroy(llx_serve* h) {
+  if (!h) return;
+  session_free(&h->s);
+  delete h;
+}
+
+llx_status llx_serve_step(llx_serve* h, int n, const int32_t* slots, const int32_t* counts, const int32_t* tokens,
+                          const llx_sampling* how, int32_t* next, float* prob, int16_t* logits) {
+  return guarded([&] {
+    require(h && slots && counts && tokens && next, LLX_ERR_INVALID, "null argument");
+    llx_session* s = &h->s;
+    llx_model* m = s->m;
+    PagedState& p = *s->paged;
+    require(n >= 1, LLX_ERR_INVALID, "a step needs a sequence");
+    paged_slots(p, n, slots, true);
+    std::vector<int32_t> starts(n + 1, 0), last(n);
+    int64_t rows = 0, pages = 0;
+    int most = 0, longest = 0;
+    for (int i = 0; i < n; ++i) {
+      const int len = p.len[slots[i]];
+      require(counts[i] >= 1, LLX_ERR_INVALID, "a sequence of a step needs a token");
+      require((int64_t)len + counts[i] <= m->max_seq, LLX_ERR_RANGE,
+              "slot " + std::to_string(slots[i]) + ": " + std::to_string((int64_t)len + counts[i]) +
+                  " positions exceed max_seq=" + std::to_string(m->max_seq));
+      rows += counts[i];
+      require(rows <= s->max_rows, LLX_ERR_RANGE, "the step's tokens exceed max_rows=" + std::to_string(s->max_rows));
+      starts[i + 1] = (int32_t)rows;
+      last[i] = (int32_t)rows - 1;
+      pages += paged_need(p, len + counts[i]) - paged_need(p, len);
+      most = std::max(most, counts[i]);
+      longest = std::max(longest, len + counts[i]);
+    }
+    for (int64_t i = 0; i < rows; ++i)
+      require(tokens[i] >= 0 && tokens[i] < m->vocab, LLX_ERR_RANGE, "token ID exceeds model vocabulary");
+    const bool sampled = how && how->random;
+    require(!sampled || m->vocab <= sample_max_vocab(), LLX_ERR_UNSUPPORTED, "the vocabulary is too large to sample from");
+    cudaSetDevice(m->device);
+    stage_tokens(s, tokens, (int)rows);
+    paged_put(s, p.slots, slots, n);
+    paged_put(s, p.counts, counts, n);
+    paged_put(s, p.starts, starts.data(), n + 1);
+    std::memcpy(s->h_rec, last.data(), sizeof(int32_t) * n);
+    LLX_CUDA(cudaMemcpyAsync(s->d_rec, s->h_rec, sizeof(int32_t) * n, cudaMemcpyHostToDevice, s->st));
+    LLX_CUDA(launch_pages_reserve(paged_pages(s, n), s->st));
+    if (pages > paged_free_at_least(p)) paged_check(s);  // nothing was taken when there were too few
+    for (int i = 0; i < n; ++i) p.len[slots[i]] += counts[i];
+    p.n = n;
+    p.rows = (int)rows;
+    p.max_rows = most;
+    p.max_len = longest;
+    const Binding bd = bind(s, false);
+    enqueue_steps(s, bd, 0, m->tail_start, (int)rows, (int)rows);
+    Binding bt = bd;
+    for (size_t t = 0; t < m->tail_inputs.size(); ++t) {
+      const int a = m->tail_inputs[t];
+      void* dst = s->arena + s->tail_off[t];
+      LLX_CUDA(launch_gather_rows(bd.p[a], dst, s->d_rec, n, m->acts[a].cols * m->acts[a].elem, s->st));
+      bt.p[a] = dst;
+      bt.rows[a] = s->tail_rows_alloc;
+    }
+    enqueue_steps(s, bt, m->tail_start, m->steps.size(), n, n);
+    const int16_t* out = (const int16_t*)bd.p[m->output_act];
+    if (!sampled) {
+      launch_output_argmax(s, out, n);
+    } else {
+      llx_sample_args a{};
+      a.logits = out;
+      a.logits_stride = m->vocab_padded;
+      a.rows = n;
+      a.vocab = m->vocab;
+      a.exponent = m->E_LOGIT;
+      auto put = [&](auto* dst, const auto* src) { paged_put(s, dst, src, src ? n : 0); };
+      put(p.random, how->random);
+      put(p.temperature, how->temperature);
+      put(p.top_k, how->top_k);
+      put(p.top_p, how->top_p);
+      put(p.min_p, how->min_p);
+      a.random = p.random;
+      a.temperature = how->temperature ? p.temperature : nullptr;
+      a.top_k = how->top_k ? p.top_k : nullptr;
+      a.top_p = how->top_p ? p.top_p : nullptr;
+      a.min_p = how->min_p ? p.min_p : nullptr;
+      a.token = s->d_argmax;
+      a.prob = p.prob;
+      LLX_CUDA(launch_sample(a, s->st));
+      if (prob) LLX_CUDA(cudaMemcpyAsync(prob, p.prob, sizeof(float) * n, cudaMemcpyDeviceToHost, s->st));
+    }
+    paged_check(s);
+    check_device_error(s);
+    copy_outputs(s, n, logits, next);
+  });
+}
+
+llx_status llx_serve_fork(llx_serve* h, int n, const int32_t* parents, const int32_t* children, int share) {
+  return guarded([&] {
+    require(h, LLX_ERR_INVALID, "null argument");
+    llx_session* s = &h->s;
+    PagedState& p = *s->paged;
+    paged_slots(p, n, parents, false);
+    paged_slots(p, n, children, true);
+    std::vector<char> is_child(p.max_seqs, 0);
+    for (int i = 0; i < n; ++i) is_child[children[i]] = 1;
+    int64_t pages = 0;
+    for (int i = 0; i < n; ++i) {
+      require(!is_child[parents[i]], LLX_ERR_INVALID, "slot " + std::to_string(parents[i]) + " is both parent and child");
+      const int len = p.len[parents[i]];
+      pages += paged_need(p, len) - (share ? len / p.page_size : 0);
+    }
+    cudaSetDevice(s->m->device);
+    paged_put(s, p.slots, parents, n);
+    paged_put(s, p.counts, children, n);
+    llx_pages_args a = paged_pages(s, n);
+    a.share = share != 0;
+    LLX_CUDA(launch_pages_fork(a, s->st));
+    if (pages > paged_free_at_least(p)) paged_check(s);
+    for (int i = 0; i < n; ++i) p.len[children[i]] = p.len[parents[i]];
+    LLX_CUDA(cudaStreamSynchronize(s->st));  // the lists are the caller's
+  });
+}
+
+llx_status llx_serve_free(llx_serve* h, int n, const int32_t* slots) {
+  return guarded([&] {
+    require(h, LLX_ERR_INVALID, "null argument");
+    llx_session* s = &h->s;
+    PagedState& p = *s->paged;
+    paged_slots(p, n, slots, true);
+    cudaSetDevice(s->m->device);
+    paged_put(s, p.slots, slots, n);
+    LLX_CUDA(launch_pages_free(paged_pages(s, n), s->st));
+    for (int i = 0; i < n; ++i) p.len[slots[i]] = 0;
+    LLX_CUDA(cudaStreamSynchronize(s->st));
+  });
+}
+
+llx_status llx_serve_compact(llx_serve* h) {
+  return guarded([&] {
+    require(h, LLX_ERR_INVALID, "null argument");
+    llx_session* s = &h->s;
+    PagedState& p = *s->paged;
+    cudaSetDevice(s->m->device);
+    llx_pages_args a = paged_pages(s, 0);
+    a.new_table = p.table;
+    a.new_refs = p.refs;
+    LLX_CUDA(launch_pages_compact(a, s->st));
+    LLX_CUDA(cudaStreamSynchronize(s->st));
+  });
+}
+
+llx_status llx_serve_usage(llx_serve* h, int32_t* lengths, int* used_pages) {
+  return guarded([&] {
+    require(h, LLX_ERR_INVALID, "null argument");
+    llx_session* s = &h->s;
+    PagedState& p = *s->paged;
+    if (lengths) std::memcpy(lengths, p.len.data(), sizeof(int32_t) * p.max_seqs);
+    if (used_pages) {
+      std::vector<int32_t> refs(p.n_pages);
+      cudaSetDevice(s->m->device);
+      LLX_CUDA(cudaMemcpyAsync(refs.data(), p.refs, sizeof(int32_t) * p.n_pages, cudaMemcpyDeviceToHost, s->st));
+      LLX_CUDA(cudaStreamSynchronize(s->st));
+      *used_pages = (int)std::count_if(refs.begin(), refs.end(), [](int32_t r) { return r > 0; });
+    }
   });
 }
 

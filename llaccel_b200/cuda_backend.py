@@ -70,6 +70,13 @@ SIGNATURES = {
     "llx_pages_free": (C.c_int, [C.c_char_p, C.c_void_p]),
     "llx_pages_compact": (C.c_int, [C.c_char_p, C.c_void_p]),
     "llx_sample": (C.c_int, [C.c_char_p, C.c_void_p]),
+    "llx_serve_create": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int, C.POINTER(C.c_void_p)]),
+    "llx_serve_destroy": (None, [C.c_void_p]),
+    "llx_serve_step": (C.c_int, [C.c_void_p, C.c_int, _I32P, _I32P, _I32P, C.c_void_p, _I32P, C.c_void_p, C.c_void_p]),
+    "llx_serve_fork": (C.c_int, [C.c_void_p, C.c_int, _I32P, _I32P, C.c_int]),
+    "llx_serve_free": (C.c_int, [C.c_void_p, C.c_int, _I32P]),
+    "llx_serve_compact": (C.c_int, [C.c_void_p]),
+    "llx_serve_usage": (C.c_int, [C.c_void_p, _I32P, C.POINTER(C.c_int)]),
 }
 
 
@@ -478,3 +485,134 @@ class CudaLanes:
     def close(self) -> None:
         for m in reversed(self.models):
             m.close()
+
+
+class LlxSampling(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("random", "temperature", "top_k", "top_p", "min_p")]
+
+
+class CudaServe:
+    """A model served over a paged KV cache (llx_serve_*): sequences of different lengths share each
+    step and one pool of pages.  `model` is a loaded CudaModel (fuse=True, one GPU), whose weights it
+    uses and which has to stay open.
+
+    `step` takes any number of new tokens per sequence and returns one next token each; `fork` lets
+    several answers go on from one prompt, `free` gives a slot back.  Tokens and logits are those of
+    CudaModel on each sequence alone, whatever else is in the step.  Too few free pages raise
+    LlxError with code LLX_ERR_OOM and change nothing."""
+
+    def __init__(self, model: CudaModel, *, max_seqs: int, n_pages: int, page_size: int = 64, max_rows: int = 1024) -> None:
+        self.model, self.lib = model, model.lib
+        self.max_seqs, self.n_pages, self.page_size, self.max_rows = int(max_seqs), int(n_pages), int(page_size), int(max_rows)
+        self._h = C.c_void_p()
+        _check(self.lib, self.lib.llx_serve_create(model._model, self.max_seqs, self.n_pages, self.page_size, self.max_rows,
+                                                   C.byref(self._h)))
+
+    def close(self) -> None:
+        if getattr(self, "_h", None):
+            self.lib.llx_serve_destroy(self._h)
+            self._h = None
+
+    def __del__(self):  # pragma: no cover
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        self.close()
+
+    @staticmethod
+    def _ints(x) -> np.ndarray:
+        return np.ascontiguousarray(np.asarray(x, dtype=np.int32).reshape(-1))
+
+    def step(self, slots, tokens, *, random=None, temperature=None, top_k=None, top_p=None, min_p=None,
+             with_logits: bool = False) -> dict:
+        """`tokens[i]`: the new tokens (one or more) of the sequence in `slots[i]`.  `random`: a number of
+        [0, 1) per sequence, to sample with the given settings (per sequence, or one for all);
+        without it the largest logit is taken.  Returns {"next": int32 [n], "prob": float32 [n] or
+        None, "logits": int16 [n, vocab_padded] or None}."""
+        slots = self._ints(slots)
+        lists = [self._ints(t) for t in tokens]
+        n = len(slots)
+        if len(lists) != n:
+            raise ValueError(f"{n} slots, but tokens of {len(lists)} sequences")
+        counts = self._ints([len(t) for t in lists])
+        flat = np.concatenate(lists) if lists else np.zeros(0, np.int32)
+        nxt, how, prob, kept = np.zeros(n, np.int32), None, None, []
+        if random is not None:
+            how = LlxSampling()
+            for name, value, kind in (("random", random, np.float64), ("temperature", temperature, np.float32),
+                                      ("top_k", top_k, np.int32), ("top_p", top_p, np.float32), ("min_p", min_p, np.float32)):
+                if value is None:
+                    continue
+                a = np.ascontiguousarray(np.broadcast_to(np.asarray(value, dtype=kind), (n,)))
+                kept.append(a)
+                setattr(how, name, a.ctypes.data)
+            prob = np.zeros(n, np.float32)
+        elif any(v is not None for v in (temperature, top_k, top_p, min_p)):
+            raise ValueError("sampling needs random numbers")
+        logits = np.empty((n, self.model.vocab_padded), np.int16) if with_logits else None
+        _check(self.lib, self.lib.llx_serve_step(self._h, n, _p32(slots), _p32(counts), _p32(flat),
+                                                 C.byref(how) if how is not None else None, _p32(nxt),
+                                                 prob.ctypes.data if prob is not None else None,
+                                                 logits.ctypes.data if logits is not None else None))
+        return {"next": nxt, "prob": prob, "logits": logits}
+
+    def fork(self, parents, children, *, share: bool = True) -> None:
+        """Slot `children[i]` becomes a copy of slot `parents[i]`: full pages shared (or, without `share`,
+        copied too), a part-filled last page copied."""
+        p, c = self._ints(parents), self._ints(children)
+        if len(p) != len(c):
+            raise ValueError("one parent per child")
+        _check(self.lib, self.lib.llx_serve_fork(self._h, len(p), _p32(p), _p32(c), 1 if share else 0))
+
+    def free(self, slots) -> None:
+        s = self._ints(slots)
+        _check(self.lib, self.lib.llx_serve_free(self._h, len(s), _p32(s)))
+
+    def compact(self) -> None:
+        """Moves the pages in use to the front of the cache."""
+        _check(self.lib, self.lib.llx_serve_compact(self._h))
+
+    def usage(self) -> tuple[np.ndarray, int]:
+        """(positions per slot, pages in use)."""
+        lengths, used = np.zeros(self.max_seqs, np.int32), C.c_int()
+        _check(self.lib, self.lib.llx_serve_usage(self._h, _p32(lengths), C.byref(used)))
+        return lengths, used.value
+
+    def generate(self, prompts, n_tokens: int, *, rng=None, chunk: int | None = None, **settings) -> list[list[int]]:
+        """`n_tokens` new tokens after each of the prompts (any lengths, at most max_seqs of them), greedy
+        or, with `rng` (a numpy Generator), sampled with `settings`.  Prompts go in by chunks of at
+        most `chunk` tokens (default: what a step's rows allow), while others already decode.  Uses
+        slots 0 .. len(prompts) - 1 and gives them back."""
+        P = [self.model._validate(p, n_tokens) for p in prompts]
+        if len(P) > self.max_seqs:
+            raise ValueError(f"{len(P)} prompts, but {self.max_seqs} slots")
+        if len(P) > self.max_rows:
+            raise ValueError(f"{len(P)} prompts, but steps of {self.max_rows} rows")
+        out: list[list[int]] = [[] for _ in P]
+        left = [list(p) for p in P]
+        self.free(range(len(P)))
+        try:
+            while n_tokens and any(len(o) < n_tokens for o in out):
+                live = [i for i, o in enumerate(out) if len(o) < n_tokens]
+                room, slots, feed = self.max_rows - len(live), [], []
+                for i in live:
+                    take = min(len(left[i]), 1 + room, chunk or len(left[i]))
+                    room -= take - 1
+                    slots.append(i)
+                    feed.append(left[i][:take])
+                    left[i] = left[i][take:]
+                extra = dict(random=rng.random(len(slots)), **settings) if rng is not None else {}
+                got = self.step(slots, feed, **extra)["next"]
+                for i, t in zip(slots, got):
+                    if not left[i]:
+                        out[i].append(int(t))
+                        left[i] = [int(t)]
+        finally:
+            self.free(range(len(P)))
+        return out
