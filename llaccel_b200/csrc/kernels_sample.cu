@@ -265,6 +265,15 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const llx_sample_args a,
   auto weight = [&](int g) {
     return small ? gap_weight<true>((uint32_t)g, set.step, sh.pow2) : gap_weight<false>((uint32_t)g, set.step, sh.pow2);
   };
+  auto weights = [&](const int (&g)[8], uint32_t (&w)[8]) {
+    if (small) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[j] = gap_weight<true>((uint32_t)g[j], set.step, sh.pow2);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[j] = gap_weight<false>((uint32_t)g[j], set.step, sh.pow2);
+    }
+  };
   // largest gap whose weight is at least `least` (weight(0) is): every warp tries 32 gaps a round
   auto farthest = [&](uint32_t least) {
     int l = 0;
@@ -305,9 +314,11 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const llx_sample_args a,
       for (int v = tid; v < nv; v += kThreads) {
         int g[8];
         gaps(v, g);
+        // weights first, choices after: no branches around the arithmetic
+        uint32_t w[8];
+        weights(g, w);
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (g[j] != kOut) sum += weight(g[j]);
+        for (int j = 0; j < 8; ++j) sum += g[j] != kOut ? w[j] : 0u;
       }
       CountSum all;
       block_prefix(CountSum{sum, 0}, sh, &all);
@@ -327,15 +338,16 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const llx_sample_args a,
       if (!near(v, reach)) continue;
       int g[8];
       gaps(v, g);
+      uint32_t w[8];
+      if (set.by_part) weights(g, w);
 #pragma unroll
       for (int j = 0; j < 8; ++j)
         if (g[j] <= reach) {
           const int b = g[j] >> s;
           if (by_k) atomicAdd(&sh.count[b], 1u);
           if (set.by_part) {
-            const uint32_t w = weight(g[j]);
-            atomicAdd(&sh.low[b], w & 0xffffu);
-            atomicAdd(&sh.high[b], w >> 16);
+            atomicAdd(&sh.low[b], w[j] & 0xffffu);
+            atomicAdd(&sh.high[b], w[j] >> 16);
           }
         }
     }
@@ -467,9 +479,11 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const llx_sample_args a,
     for (int j = 0; j < 8; ++j) g[j] = kOut;
     if (!near(v, G)) return t;
     gaps(v, g);
+    uint32_t w[8];
+    weights(g, w);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      if (g[j] < G) t.sum += weight(g[j]);
+      t.sum += g[j] < G ? w[j] : 0u;
       t.count += g[j] == G;
     }
     return t;
