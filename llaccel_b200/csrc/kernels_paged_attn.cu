@@ -145,7 +145,9 @@ cudaError_t make_page_map(CUtensorMap* map, const void* base, const llx_paged_at
   return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
-cudaError_t launch_paged_attention(const llx_paged_attention_args& a, cudaStream_t st) {
+cudaError_t launch_paged_attention(const llx_paged_attention_args& args, cudaStream_t st) {
+  llx_paged_attention_args a = args;
+  if (a.max_rows > a.rows) a.max_rows = a.rows;  // grids follow it
   if (a.rows == 0 || a.n_seqs == 0 || a.max_rows == 0) return cudaSuccess;
   const int64_t pairs = a.max_rows * (a.n_heads / a.n_kv_heads);
   // Up to 32 stacked pairs the cache is read once per 8 of them by the few-row kernel; from there on,

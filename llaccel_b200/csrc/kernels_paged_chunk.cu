@@ -108,6 +108,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   unsigned char* base = raw + ((1024 - (pa::s32(raw) & 1023)) & 1023);
   for (int x = tid; x < 1024; x += kThreads)
     reinterpret_cast<uint4*>(base + L::curve)[x] = reinterpret_cast<const uint4*>(kDevCurve)[x];
+  __syncthreads();  // any_bad is clear before a thread sets it
   pdl_trigger();
   pdl_wait();
   const int i = blockIdx.z, kvh = blockIdx.y;
