@@ -23,17 +23,18 @@
 
 namespace llx {
 
-// SMALL: step < 2^28, so e stays in 32 bits (g is below 2^16).
+// The weight of gap g, 0 from `limit` on.  SMALL: step < 2^28, so e stays in 32 bits (g is below 2^16).
 template <bool SMALL>
-__device__ __forceinline__ uint32_t gap_weight(uint32_t g, uint64_t step, const uint32_t* pow2) {
+__device__ __forceinline__ uint32_t gap_weight(uint32_t g, uint64_t step, const uint32_t* pow2, uint32_t limit = ~0u) {
   uint32_t e, n;
   if (SMALL) {
-    e = (uint32_t)(((uint64_t)g * (uint32_t)step) >> 12);
+    e = __umulhi(g << 16, (uint32_t)step << 4);  // (g * step) >> 12
+    if (g >= limit) e = 32u << 20;  // and all such lanes look up the same entry
     n = e >> 20;
   } else {
     const uint64_t x = (g * step) >> 12;
     e = (uint32_t)x;
-    n = x >> 20 < 32 ? (uint32_t)(x >> 20) : 32u;
+    n = x >> 20 < 32 && g < limit ? (uint32_t)(x >> 20) : 32u;
   }
   const uint32_t b = pow2[(e >> 10) & 1023u];
   uint32_t w;
@@ -53,12 +54,16 @@ __device__ __forceinline__ uint64_t part_ceil(uint64_t total, uint32_t f) {
 // what one row's settings come to
 struct SampleRow {
   uint64_t step;
-  int64_t k;       // tokens top-k keeps
   uint32_t part;   // top-p in units of 2^-31
-  bool by_part;
   uint32_t least;  // min-p's smallest weight
   uint32_t u;      // random number in units of 2^-31
 };
+
+__device__ __forceinline__ int64_t row_k(const llx_sample_args& a, int64_t r) {
+  if (a.temperature && !(a.temperature[r] > 0.0f)) return 1;
+  const int k = a.top_k ? a.top_k[r] : 0;
+  return k <= 0 || k > a.vocab ? a.vocab : k;
+}
 
 __device__ __forceinline__ SampleRow sample_row(const llx_sample_args& a, int64_t r) {
   SampleRow s;
@@ -68,10 +73,7 @@ __device__ __forceinline__ SampleRow sample_row(const llx_sample_args& a, int64_
   const double unit = scalbn(1.4426950408889634, (int)(32 + a.exponent));
   const double q = greedy ? 0.0 : rint(unit / (double)temp);
   s.step = q >= 140737488355328.0 ? 1ull << 47 : (uint64_t)q;
-  const int k = a.top_k ? a.top_k[r] : 0;
-  s.k = greedy ? 1 : (k <= 0 || k > a.vocab ? a.vocab : k);
   const float p = a.top_p ? a.top_p[r] : 1.0f;
-  s.by_part = p < 1.0f;
   s.part = !(p > 0.0f) ? 0u : p >= 1.0f ? 1u << 31 : (uint32_t)((double)p * 2147483648.0);
   const float m = a.min_p ? a.min_p[r] : 0.0f;
   s.least = !(m > 0.0f) ? 0u : m >= 1.0f ? 1u << 31 : (uint32_t)ceil((double)m * 2147483648.0);
@@ -85,17 +87,26 @@ __device__ __forceinline__ SampleRow sample_row(const llx_sample_args& a, int64_
 // logits are read from memory once; every decision is made by all CTAs alike from what they
 // exchange (integer counts and sums: the order of the atomics does not matter).
 //
-// The cut is found with a histogram of gaps in up to 1024 bins of 2^s levels, then one of the levels
-// of the bin it falls into.  Counting every token would cost three shared-memory atomics each, most of
-// them for the row's bulk far below the cut, so only tokens that can matter are counted:
-//   top-k  as many of the threads' own maxima as k lie above some gap, so the k-th token does too
-//          (k at most the cluster's threads);
-//   top-p  tokens of weight at most (W - need) / V add up to W - need at most, so the prefix that
-//          reaches `need` has only heavier ones.
+// Top-k first looks at the threads' own maxima, binned while the row is loaded (by level: the largest
+// logit is not known yet): as many of them as k lie above some gap, so the k-th token does too (k at
+// most the cluster's threads).  Where the tokens up to that gap are few, as they are for the usual k, the
+// cluster's first CTA gathers them, orders them by counting and finishes the row, and the others leave:
+// 22 us for 128 rows of 151,936 tokens and k = 50 (reading them takes 6), against 45 with the histogram.
+//
+// Otherwise the cut is found with a histogram of gaps in up to 1024 bins of 2^s levels, then one of the
+// levels of the bin it falls into.  Counting every token would cost three shared-memory atomics each, most
+// of them for the row's bulk far below the cut, so only tokens that can matter are counted: for top-k those
+// up to the gap above, for top-p those heavier than (W - need) / V, because the tokens up to that weight
+// add up to W - need at most and the prefix that reaches `need` has only heavier ones.
+// What bounds it: reading and a row's chain of exchanges (some 2,000 cycles each) for small k, 22 us for
+// a single row; instructions where top-p looks at a whole row, 111 a token and 113 us for 128 such rows,
+// 44 without any filter.  A window of exact levels around a cut estimated from a sample of the tokens saves
+// the atomics, but its pass does more per token: 155 us.
 // ---------------------------------------------------------------------------------------
 constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kBins = 2 * kThreads;      // two per thread
-constexpr int kFirst = 256;
+constexpr int kMaxBins = kThreads;       // of the threads' maxima: 128 levels each, one per thread
+constexpr int kList = kThreads;          // candidates that one CTA finishes alone
 constexpr int kMaxCluster = 16;
 constexpr int kSliceVecs = 6400;         // 51,200 tokens: a bin's 16-bit halves of weights stay in 32 bits
 constexpr int kOut = 1 << 20;            // gap of a place that holds no token
@@ -121,25 +132,33 @@ __device__ __forceinline__ uint64_t peer_u64(const void* local, int rank) {
 }
 
 struct SampleShared {
-  uint32_t count[kBins], low[kBins], high[kBins];  // gaps: tokens, their weights' lower and upper 16 bits
-  uint64_t added[3][kBins / 4];                    // this CTA's share of the bins, of all CTAs (4 or more)
-  uint32_t first[kFirst];                          // gaps of the threads' maxima, 256 levels a bin
-  uint32_t level[2][64];                           // tokens per level of a bin: for top-k, for top-p
+  union {
+    struct {
+      uint32_t count[kBins], low[kBins], high[kBins];  // gaps: tokens, their weights' lower and upper 16 bits
+    };
+    struct {  // of the CTA that finishes a row from its candidates
+      uint64_t keys[kList], kept[kList];
+    };
+  };
+  uint64_t added[3][kBins / 4];  // this CTA's share of the bins, of all CTAs (4 or more)
+  uint32_t level[2][64];         // tokens per level of a bin: for top-k, for top-p
+  uint64_t list[kList];          // this CTA's candidates: gap and token
+  uint32_t most[kMaxBins];       // the threads' maxima
   uint32_t pow2[1024];
   uint64_t warp_sum[kWarps];
   uint32_t warp_count[kWarps];
   SampleRow set;
   // read by the peers
   int32_t max;
+  uint32_t listed;
   uint64_t whole;
-  uint64_t kept;
+  uint64_t kept_sum;
   uint32_t ties;
   // this CTA's decisions
   int32_t bin[3];
   uint64_t below_sum[3];
   uint32_t below_count[3];
   int32_t gap;
-  int64_t take;
 };
 
 template <int C>
@@ -150,12 +169,10 @@ __device__ __forceinline__ void cluster_meet() {
     __syncthreads();
 }
 
-// exclusive prefix over the block's threads, and the whole
-__device__ __forceinline__ CountSum block_prefix(CountSum v, SampleShared& sh, CountSum* whole) {
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  CountSum s = v;
+__device__ __forceinline__ CountSum warp_scan(CountSum s, int width) {  // inclusive
+  const int lane = threadIdx.x & 31;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
+  for (int o = 1; o < width; o <<= 1) {
     const uint64_t ys = __shfl_up_sync(0xffffffffu, s.sum, o);
     const uint32_t yc = __shfl_up_sync(0xffffffffu, s.count, o);
     if (lane >= o) {
@@ -163,21 +180,63 @@ __device__ __forceinline__ CountSum block_prefix(CountSum v, SampleShared& sh, C
       s.count += yc;
     }
   }
+  return s;
+}
+
+// exclusive prefix over the block's threads, and the whole
+__device__ __forceinline__ CountSum block_prefix(CountSum v, SampleShared& sh, CountSum* whole) {
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const CountSum s = warp_scan(v, 32);
   __syncthreads();
   if (lane == 31) {
     sh.warp_sum[w] = s.sum;
     sh.warp_count[w] = s.count;
   }
   __syncthreads();
-  CountSum before{0, 0}, all{0, 0};
-#pragma unroll
-  for (int x = 0; x < kWarps; ++x) {
-    if (x == w) before = all;
-    all.sum += sh.warp_sum[x];
-    all.count += sh.warp_count[x];
+  // every warp scans the warps' sums itself
+  const CountSum all = warp_scan(lane < kWarps ? CountSum{sh.warp_sum[lane], sh.warp_count[lane]} : CountSum{0, 0}, kWarps);
+  const uint64_t before_sum = __shfl_sync(0xffffffffu, all.sum, (w + 31) & 31);
+  const uint32_t before_count = __shfl_sync(0xffffffffu, all.count, (w + 31) & 31);
+  *whole = CountSum{__shfl_sync(0xffffffffu, all.sum, kWarps - 1), __shfl_sync(0xffffffffu, all.count, kWarps - 1)};
+  return CountSum{(w ? before_sum : 0) + s.sum - v.sum, (w ? before_count : 0) + s.count - v.count};
+}
+
+// A row's draw from its candidates, one per thread (gap and token, n of them; they hold the k first).
+template <class Weight>
+__device__ __forceinline__ void draw_from_list(const llx_sample_args& a, int64_t r, uint64_t key, int n, int k, bool by_part,
+                                               const SampleRow& set, Weight weight, SampleShared& sh) {
+  const int tid = threadIdx.x;
+  uint64_t* keys = sh.keys;
+  uint64_t* kept = sh.kept;  // in order: weight and token
+  keys[tid] = key;
+  if (tid == 0) sh.bin[0] = k;
+  __syncthreads();
+  int place = 0;  // in the order of gap and index
+  const uint32_t w = tid < n ? weight((int)(key >> 32)) : 0;
+  if (tid < n) {
+    for (int j = 0; j < n; ++j) place += keys[j] < key;
+    kept[place] = (uint64_t)w << 32 | (uint32_t)key;
   }
-  *whole = all;
-  return CountSum{before.sum + s.sum - v.sum, before.count + s.count - v.count};
+  __syncthreads();
+  const uint64_t s = tid < k ? kept[tid] >> 32 : 0;
+  CountSum whole;
+  const CountSum at = block_prefix(CountSum{s, 0}, sh, &whole);
+  const uint64_t need = max(part_ceil(whole.sum, set.part), (uint64_t)1);
+  if (by_part && at.sum < need && at.sum + s >= need) sh.bin[0] = tid + 1;
+  const int heavy = __syncthreads_count(tid < n && w >= set.least);
+  const int last = min(sh.bin[0], heavy);
+  if (place >= last || tid >= n) return;
+  uint64_t start = 0, total = 0;
+  for (int j = 0; j < last; ++j) {
+    const uint64_t x = kept[j];
+    total += x >> 32;
+    start += (uint32_t)x < (uint32_t)key ? x >> 32 : 0;
+  }
+  const uint64_t target = part_floor(total, set.u);
+  if (start <= target && target < start + w) {
+    a.token[r] = (int)(uint32_t)key;
+    if (a.prob) a.prob[r] = (float)((double)w / (double)total);
+  }
 }
 
 template <int C>
@@ -188,9 +247,10 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const llx_sample_args a,
   const int64_t r = blockIdx.x / C;
   const int rank = (int)(blockIdx.x % C);
   for (int x = tid; x < kBins; x += kThreads) sh.count[x] = sh.low[x] = sh.high[x] = 0;
-  if (tid < kFirst) sh.first[tid] = 0;
-  for (int x = tid; x < 1024; x += kThreads) sh.pow2[x] = kDevPow2[x];
+  sh.most[tid] = 0;
   if (tid < 64) sh.level[0][tid] = sh.level[1][tid] = 0;
+  if (tid == 0) sh.listed = 0;
+  for (int x = tid; x < 1024; x += kThreads) sh.pow2[x] = kDevPow2[x];
   pdl_trigger();
   pdl_wait();
   // The row lies in 16-byte vectors from the one that holds its first token on; this CTA has the
@@ -201,42 +261,42 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const llx_sample_args a,
   const int v0 = rank * slice, nv = max(0, min(slice, (skew + V + 7) / 8 - v0));
   const int lo = max(0, skew - v0 * 8), hi = min(nv * 8, skew + V - v0 * 8);
   const int16_t* from = row - skew + (int64_t)v0 * 8;
-  int mine = -32768;
-  bool any = false;
+  const int64_t k = row_k(a, r);
+  const bool by_k = k < V, by_part = a.top_p && a.top_p[r] < 1.0f;
+  auto bin_at = [](int level) { return (level + 32768) >> 7; };
+  if (by_k) __syncthreads();  // the counts are clear
+  uint32_t most = 0x80008000u;  // of the thread's tokens
   for (int v = tid; v < nv; v += kThreads) {
     uint4 x;
-    int16_t* e = reinterpret_cast<int16_t*>(&x);
     if (v * 8 >= lo && v * 8 + 8 <= hi) {
       x = reinterpret_cast<const uint4*>(from)[v];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) mine = max(mine, (int)e[j]);
-      any = true;
     } else {
       x = make_uint4(0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u);
+      int16_t* e = reinterpret_cast<int16_t*>(&x);
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (v * 8 + j >= lo && v * 8 + j < hi) {
-          e[j] = from[v * 8 + j];
-          mine = max(mine, (int)e[j]);
-          any = true;
-        }
+        if (v * 8 + j >= lo && v * 8 + j < hi) e[j] = from[v * 8 + j];
     }
     vecs[v] = x;
+    most = __vmaxs2(most, __vmaxs2(__vmaxs2(x.x, x.y), __vmaxs2(x.z, x.w)));
   }
+  const int mine = max((int)(int16_t)(most & 0xffffu), (int)most >> 16);
+  const bool any = tid < nv;  // every vector has a token
+  if (by_k && any) atomicAdd(&sh.most[bin_at(mine)], 1u);
   // one thread works out the row's settings (doubles) while the others load
   if (tid == kThreads - 1) sh.set = sample_row(a, r);
   {
-    const int m = __reduce_max_sync(0xffffffffu, any ? mine : INT_MIN);
+    const int m = __reduce_max_sync(0xffffffffu, mine);
     if (lane == 0) sh.warp_count[warp] = (uint32_t)m;
     __syncthreads();
     if (warp == 0) {
-      const int x = __reduce_max_sync(0xffffffffu, lane < kWarps ? (int)sh.warp_count[lane] : INT_MIN);
+      const int x = __reduce_max_sync(0xffffffffu, lane < kWarps ? (int)sh.warp_count[lane] : -32768);
       if (lane == 0) sh.max = x;
     }
   }
   cluster_meet<C>();
   const SampleRow set = sh.set;
-  int mx = INT_MIN;
+  int mx = -32768;
 #pragma unroll
   for (int c = 0; c < C; ++c) mx = max(mx, C > 1 ? (int)peer_u32(&sh.max, c) : sh.max);
 
@@ -265,13 +325,14 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const llx_sample_args a,
   auto weight = [&](int g) {
     return small ? gap_weight<true>((uint32_t)g, set.step, sh.pow2) : gap_weight<false>((uint32_t)g, set.step, sh.pow2);
   };
-  auto weights = [&](const int (&g)[8], uint32_t (&w)[8]) {
+  // weights first, choices after: no branches around the arithmetic
+  auto weights = [&](const int (&g)[8], uint32_t (&w)[8], int limit) {
     if (small) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) w[j] = gap_weight<true>((uint32_t)g[j], set.step, sh.pow2);
+      for (int j = 0; j < 8; ++j) w[j] = gap_weight<true>((uint32_t)g[j], set.step, sh.pow2, (uint32_t)limit);
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) w[j] = gap_weight<false>((uint32_t)g[j], set.step, sh.pow2);
+      for (int j = 0; j < 8; ++j) w[j] = gap_weight<false>((uint32_t)g[j], set.step, sh.pow2, (uint32_t)limit);
     }
   };
   // largest gap whose weight is at least `least` (weight(0) is): every warp tries 32 gaps a round
@@ -288,37 +349,62 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const llx_sample_args a,
     return l;
   };
 
-  const bool by_k = set.k < V;
   int G = 65535;       // kept: gaps below G and `take` tokens of gap G
   int64_t take = V;
-  if (by_k || set.by_part) {
+  if (by_k || by_part) {
     int reach = 65535;  // no token beyond this gap matters
     if (by_k) {
-      if (set.k <= (int64_t)kThreads * C) {
-        if (any) atomicAdd(&sh.first[(mx - mine) >> 8], 1u);
-        cluster_meet<C>();
+      if (k <= (int64_t)kThreads * C) {
+        // bin d from the largest logit's down holds the gaps (off + 128 (d - 1), off + 128 d]
+        const int top = bin_at(mx), off = (mx + 32768) & 127;
         uint32_t n = 0;
-        if (tid < kFirst)
+        if (tid <= top)
 #pragma unroll
-          for (int c = 0; c < C; ++c) n += C > 1 ? peer_u32(&sh.first[tid], c) : sh.first[tid];
+          for (int c = 0; c < C; ++c) n += C > 1 ? peer_u32(&sh.most[top - tid], c) : sh.most[top - tid];
         CountSum all;
         const CountSum at = block_prefix(CountSum{0, n}, sh, &all);
-        if (tid == 0) sh.bin[2] = kFirst - 1;
+        if (tid == 0) sh.bin[2] = kMaxBins - 1;
         __syncthreads();
-        if (at.count < set.k && at.count + n >= set.k) sh.bin[2] = tid;
+        if (at.count < k && at.count + n >= k) sh.bin[2] = tid;
         __syncthreads();
-        reach = sh.bin[2] * 256 + 255;
+        reach = min(reach, off + 128 * sh.bin[2]);
+        if (k <= kList / 2) {
+          for (int v = tid; v < nv; v += kThreads) {
+            if (!near(v, reach)) continue;
+            int g[8];
+            gaps(v, g);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              if (g[j] <= reach) {
+                const uint32_t x = atomicAdd(&sh.listed, 1u);
+                if (x < kList) sh.list[x] = (uint64_t)g[j] << 32 | (uint32_t)((v0 + v) * 8 + j - skew);
+              }
+          }
+          cluster_meet<C>();
+          uint64_t key = ~0ull;
+          uint32_t n = 0;
+#pragma unroll
+          for (int c = 0; c < C; ++c) {
+            const uint32_t m = C > 1 ? peer_u32(&sh.listed, c) : sh.listed;
+            if (rank == 0 && tid >= n && tid < n + m && tid - n < kList) key = C > 1 ? peer_u64(&sh.list[tid - n], c) : sh.list[tid - n];
+            n += m;
+          }
+          if (n <= kList) {
+            if (C > 1) cluster_meet<C>();  // the first CTA has them all
+            if (rank == 0) draw_from_list(a, r, key, (int)n, (int)k, by_part, set, weight, sh);
+            return;
+          }
+        }
       }
     } else {
       uint64_t sum = 0;
       for (int v = tid; v < nv; v += kThreads) {
         int g[8];
         gaps(v, g);
-        // weights first, choices after: no branches around the arithmetic
         uint32_t w[8];
-        weights(g, w);
+        weights(g, w, kOut);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) sum += g[j] != kOut ? w[j] : 0u;
+        for (int j = 0; j < 8; ++j) sum += w[j];
       }
       CountSum all;
       block_prefix(CountSum{sum, 0}, sh, &all);
@@ -339,13 +425,13 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const llx_sample_args a,
       int g[8];
       gaps(v, g);
       uint32_t w[8];
-      if (set.by_part) weights(g, w);
+      if (by_part) weights(g, w, kOut);
 #pragma unroll
       for (int j = 0; j < 8; ++j)
         if (g[j] <= reach) {
           const int b = g[j] >> s;
           if (by_k) atomicAdd(&sh.count[b], 1u);
-          if (set.by_part) {
+          if (by_part) {
             atomicAdd(&sh.low[b], w[j] & 0xffffu);
             atomicAdd(&sh.high[b], w[j] >> 16);
           }
@@ -444,12 +530,12 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const llx_sample_args a,
     };
     uint64_t total = all.sum;
     if (by_k) {
-      cut(0, [&](const CountSum& v) { return (int64_t)v.count >= set.k; });
+      cut(0, [&](const CountSum& v) { return (int64_t)v.count >= k; });
       G = sh.gap;
-      take = set.k - (int64_t)sh.below_count[2];
+      take = k - (int64_t)sh.below_count[2];
       total = sh.below_sum[2] + (uint64_t)take * weight(G);
     }
-    if (set.by_part) {
+    if (by_part) {
       if (!by_k) {
         total = 0;
 #pragma unroll
@@ -480,10 +566,10 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const llx_sample_args a,
     if (!near(v, G)) return t;
     gaps(v, g);
     uint32_t w[8];
-    weights(g, w);
+    weights(g, w, G);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      t.sum += g[j] < G ? w[j] : 0u;
+      t.sum += w[j];
       t.count += g[j] == G;
     }
     return t;
@@ -498,7 +584,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const llx_sample_args a,
   CountSum here;  // this CTA's
   const CountSum ahead = block_prefix(own, sh, &here);
   if (tid == 0) {
-    sh.kept = here.sum;
+    sh.kept_sum = here.sum;
     sh.ties = here.count;
   }
   cluster_meet<C>();
@@ -506,9 +592,10 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const llx_sample_args a,
 #pragma unroll
   for (int c = 0; c < C; ++c) {
     if (c == rank) before = all;
-    all.sum += C > 1 ? peer_u64(&sh.kept, c) : sh.kept;
+    all.sum += C > 1 ? peer_u64(&sh.kept_sum, c) : sh.kept_sum;
     all.count += C > 1 ? peer_u32(&sh.ties, c) : sh.ties;
   }
+  if (C > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // nothing more is read from a peer
   before.sum += ahead.sum;
   before.count += ahead.count;
   const int64_t ties = min(take, (int64_t)all.count);
@@ -556,7 +643,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const llx_sample_args a,
   }
   if (C > 1) {  // no CTA leaves while a peer may still read from it
     __syncwarp();
-    cluster_meet<C>();
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   }
 }
 
