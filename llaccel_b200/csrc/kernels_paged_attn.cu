@@ -21,7 +21,9 @@ __device__ __forceinline__ T reduce_block(T v, T* scratch, Op op) {
   return r;
 }
 
-// Any geometry: one block per (row, query head), three passes over the keys, scores recomputed.
+// Any geometry (head sizes other than 64 and 128, more sequences than a grid axis holds): one block per
+// (row, query head), three passes over the keys, scores recomputed.  It reads a row's keys three times for
+// every query head and has no reuse between rows: 57.7 ms where the chunk kernel takes 0.27.
 __global__ void __launch_bounds__(256) k_paged_attention_any(const llx_paged_attention_args a) {
   pdl_trigger();
   pdl_wait();

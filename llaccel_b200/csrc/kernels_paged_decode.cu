@@ -1,9 +1,9 @@
 // Paged attention of few query rows per sequence (decode steps, a handful of draft tokens).
 //
 // A cluster of C CTAs serves one (sequence, KV head, group of up to 8 stacked (row, head) pairs);
-// each CTA takes a slice of the keys.  One thread streams the slice's K rows, then its V rows,
-// page by page through a ring of TMA-filled stages; eight warps consume them, so every byte of the
-// cache is read once:
+// each CTA takes a slice of the keys.  Two warps stream the slice's K rows, then its V rows, page by
+// page through a ring of TMA-filled stages (one warp: 84 us and 112 for the
+// launches below); eight warps consume them, so every byte of the cache is read once:
 //   scores  S^T (16 keys x 8 pairs) = K (16 x 32) Q^T per int8 MMA, kept in shared memory;
 //   maxima  of the slices meet in every CTA of the cluster (the reference's global maximum);
 //   table exponentials in place, and their sums meet the same way;
@@ -11,6 +11,13 @@
 //           the way into the MMA as two unsigned bytes, O = 256 hi + lo;
 //   partial outputs are added by the CTA that finishes them, 1/C of the outputs each.
 // Integer maxima and sums: any split gives the same bits.
+//
+// Bytes bound it.  64 sequences of 1500 to 4200 keys, 8 KV heads of 128: 80.6 us for 361 MB, 4.5 TB/s,
+// 0.68 of the copy rate; what is missing are the phases of a CTA that its neighbour on the SM does not
+// cover (1.7 waves of two CTAs an SM).  Two sequences of 64k keys: 103 us for 255 MB, 2.5 TB/s: a CTA
+// then holds its slice's scores (16 KB a thousand keys at four pairs) next to its ring and has its SM to
+// itself, the 16 clusters of 7 to 10 CTAs do not all fit at once, and a wave's exchanges have nothing to
+// hide behind.
 #include <atomic>
 #include <mutex>
 
@@ -464,8 +471,8 @@ static cudaError_t launch_decode_t(const llx_paged_attention_args& a, cudaStream
   const int64_t units = a.n_seqs * a.n_kv_heads * groups;
   // How many CTAs share a sequence's keys, and how deep their rings are: the cheapest by this count
   // (bytes and ns).  A wave takes what HBM needs for its bytes (6.5 KB a ns), or what its CTAs do: a
-  // ring's bytes per 1.9 us of loaded latency, 49 B a ns of an SM with one CTA on it, 60 with more.  A wave's phases cost 6 us where a CTA is
-  // alone on its SM, less where others stream meanwhile.  Measured: 64 sequences of 1500 to 4200 keys,
+  // ring's bytes per 1.9 us of loaded latency, 49 B a ns of an SM with one CTA on it, 60 with more.  A
+  // wave's phases cost 6 us where a CTA is alone on its SM, less where others stream meanwhile.  Measured: 64 sequences of 1500 to 4200 keys,
   // 8 KV heads: one CTA each, ring of 4 82 us, of 2 106; two CTAs, ring of 4 95, of 2 112.  Two of 64k
   // keys: 10 CTAs, ring of 6 103 us; 9, 6 113; 16, 2 118; 8, 4 127.
   double best = 1e30;
