@@ -1,4 +1,5 @@
-"""Builds the CUDA backend in-tree: llaccel_b200/csrc/*.cu -> llaccel_b200/_lib/libllx.so.
+"""Builds the CUDA backend in-tree: llaccel_b200/csrc/*.cu -> llaccel_b200/_lib/libllx.so, and where
+torch is installed the binding of the paged calls, csrc/torch_calls.cpp -> _lib/torch_calls.so.
 
     python -m llaccel_b200.build [--force]
 
@@ -10,16 +11,19 @@ from __future__ import annotations
 
 import argparse
 import fcntl
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 LIBDIR = PKG / "_lib"
 LIB = LIBDIR / "libllx.so"
+CALLS = LIBDIR / "torch_calls.so"
 INCLUDE = PKG.parent / "include"
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -43,11 +47,25 @@ def deps() -> list[Path]:
         sorted(INCLUDE.glob("*.h"))
 
 
-def up_to_date() -> bool:
-    if not LIB.exists():
+def _newer(lib: Path, sources: list[Path]) -> bool:
+    if not lib.exists():
         return False
-    t = LIB.stat().st_mtime
-    return all(p.stat().st_mtime <= t for p in deps())
+    t = lib.stat().st_mtime
+    return all(p.stat().st_mtime <= t for p in sources)
+
+
+def lib_up_to_date() -> bool:
+    return _newer(LIB, deps())
+
+
+def calls_up_to_date() -> bool:
+    if importlib.util.find_spec("torch") is None:
+        return True
+    return _newer(CALLS, [CSRC / "torch_calls.cpp", *INCLUDE.glob("*.h")])
+
+
+def up_to_date() -> bool:
+    return lib_up_to_date() and calls_up_to_date()
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
@@ -62,7 +80,11 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         try:
             if not force and up_to_date():
                 return LIB
-            return _compile(verbose)
+            if force or not lib_up_to_date():
+                _compile(verbose)
+            if force or not calls_up_to_date():
+                _compile_calls(verbose)
+            return LIB
         finally:
             fcntl.flock(lock, fcntl.LOCK_UN)
 
@@ -90,6 +112,26 @@ def _compile(verbose: bool) -> Path:
     os.replace(tmp, LIB)
     shutil.rmtree(objdir, ignore_errors=True)
     return LIB
+
+
+def _compile_calls(verbose: bool) -> None:
+    if importlib.util.find_spec("torch") is None:
+        return
+    import torch
+
+    root = Path(torch.__file__).parent
+    tmp = CALLS.with_suffix(f".so.{os.getpid()}.tmp")
+    cuda = Path(nvcc()).resolve().parent.parent
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-I", str(root / "include"), "-I", str(root / "include/torch/csrc/api/include"), "-I", str(cuda / "include"),
+           "-I", sysconfig.get_paths()["include"], str(CSRC / "torch_calls.cpp"), "-o", str(tmp), "-L", str(root / "lib"),
+           "-ltorch_python", "-ltorch_cpu", "-lc10_cuda", "-lc10"]
+    if verbose:
+        print(" ".join(cmd))
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed on torch_calls.cpp:\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, CALLS)
 
 
 def main(argv=None) -> None:

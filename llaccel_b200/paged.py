@@ -23,7 +23,10 @@ stream.  There is no CPU fallback.
 """
 from __future__ import annotations
 
+import ctypes
+import importlib.util
 import struct
+from pathlib import Path
 
 import torch
 
@@ -47,18 +50,25 @@ _I8, _I16, _I32 = torch.int8, torch.int16, torch.int32
 _stream = torch._C._cuda_getCurrentRawStream
 
 
-_lib = None
+_lib = _calls = None
 
 
 def _load():
-    global _lib
+    """libllx.so, and the binding that packs a call's tensors (torch_calls.cpp) with the calls' addresses."""
+    global _lib, _calls, _append_at, _attention_at
     _lib = load_library()
+    path = Path(__file__).resolve().parent / "_lib" / "torch_calls.so"
+    if not path.exists():
+        raise RuntimeError(f"binding missing: {path} (build it with `python -m llaccel_b200.build`)")
+    spec = importlib.util.spec_from_file_location("torch_calls", path)
+    _calls = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(_calls)
+    _append_at, _attention_at = (ctypes.cast(f, ctypes.c_void_p).value for f in (_lib.llx_paged_append, _lib.llx_paged_attention))
     return _lib
 
 
 def _refuse(dev: int, dtype, **tensors) -> None:
-    """Says which tensor (None allowed) is not on CUDA device `dev` or has another type.  Called when
-    a quick look over all of them found one; the quick looks keep a call's cost to a few us."""
+    """Says which tensor (None allowed) is not on CUDA device `dev` or has another type."""
     for name, t in tensors.items():
         if t is not None and t.dtype is not dtype:
             raise ValueError(f"{name} must be {dtype}, not {t.dtype}")
@@ -142,15 +152,24 @@ def append(q, k, v, k_pages, v_pages, table, length, q_start, cos, sin, q_rq, k_
     [positions, head_dim / 2]) and requantization by `q_rq` / `k_rq` = (M, S).  Keys and values go
     to the pages of their positions.  Returns the int8 queries, in `out` if given; rows behind
     `q_start[-1]` are left as they were."""
+    lib = _lib or _load()
+    if out is None:
+        out = torch.zeros(q.shape, dtype=_I8, device=q.device)
+    code = _calls.append(_append_at, q, k, v, k_pages, v_pages, table, length, q_start, cos, sin, q_rq, k_rq, q_norm, k_norm, seqs,
+                         out, status)
+    if code is None:  # something unusual, or wrong
+        code = _append_checked(q, k, v, k_pages, v_pages, table, length, q_start, cos, sin, q_rq, k_rq, q_norm, k_norm, seqs, out,
+                               status)
+    if code:
+        _check_code(lib, code)
+    return out
+
+
+def _append_checked(q, k, v, k_pages, v_pages, table, length, q_start, cos, sin, q_rq, k_rq, q_norm, k_norm, seqs, out, status) -> int:
     dev = _cuda(q, "q")
-    if (not (q.dtype is k.dtype is cos.dtype is sin.dtype is _I16) or not (v.dtype is k_pages.dtype is v_pages.dtype is _I8)
-            or not (table.dtype is length.dtype is q_start.dtype is _I32)
-            or not (dev == k.get_device() == v.get_device() == k_pages.get_device() == v_pages.get_device()
-                    == table.get_device() == length.get_device() == q_start.get_device() == cos.get_device()
-                    == sin.get_device()) or out is not None or seqs is not None or status is not None):
-        _refuse(dev, _I16, q=q, k=k, cos=cos, sin=sin)
-        _refuse(dev, _I8, v=v, k_pages=k_pages, v_pages=v_pages, out=out)
-        _refuse(dev, _I32, table=table, length=length, q_start=q_start, seqs=seqs, status=status)
+    _refuse(dev, _I16, q=q, k=k, cos=cos, sin=sin)
+    _refuse(dev, _I8, v=v, k_pages=k_pages, v_pages=v_pages, out=out)
+    _refuse(dev, _I32, table=table, length=length, q_start=q_start, seqs=seqs, status=status)
     if len(q.shape) != 3 or len(k_pages.shape) != 4:
         raise ValueError("q must be [rows, n_heads, head_dim], k_pages [n_pages, n_kv_heads, page_size, head_dim]")
     R, H, D = q.shape
@@ -160,8 +179,6 @@ def append(q, k, v, k_pages, v_pages, table, length, q_start, cos, sin, q_rq, k_
     rot = cos.shape
     if len(rot) != 2 or rot != sin.shape or rot[1] != D // 2 or not (cos.is_contiguous() and sin.is_contiguous()):
         raise ValueError(f"cos and sin must be dense [positions, {D // 2}]")
-    if out is None:
-        out = torch.zeros((R, H, D), dtype=_I8, device=k_pages.device)
     starts, slots, n = _launch(q_start, seqs)
     _need_slots(seqs, n, table)
     qg, qe, qC, qsh = _norm(q_norm, "q_norm", dev, D)
@@ -171,11 +188,7 @@ def append(q, k, v, k_pages, v_pages, table, length, q_start, cos, sin, q_rq, k_
                         qe, qC, qsh, ke, kC, ksh, cos.data_ptr(), sin.data_ptr(), rot[0], *q_rq, *k_rq,
                         k_pages.data_ptr(), v_pages.data_ptr(), page_stride, n_pages, P, *_table(table, length),
                         length.data_ptr(), starts, slots, n, status.data_ptr() if status is not None else 0, dev)
-    lib = _lib or _load()
-    code = lib.llx_paged_append(args, _stream(dev))
-    if code:
-        _check_code(lib, code)
-    return out
+    return (_lib or _load()).llx_paged_append(args, _stream(dev))
 
 
 def attention(q8, k_pages, v_pages, table, length, q_start, score_rq, out_rq, *, prob_bits=15, max_rows, max_len,
@@ -187,31 +200,37 @@ def attention(q8, k_pages, v_pages, table, length, q_start, score_rq, out_rq, *,
     `max_rows` and `max_len` bound every sequence's new rows and its length: what is beyond them is
     not computed.  Keys whose page id lies outside the cache count as absent; a row without keys
     gets zeros."""
+    lib = _lib or _load()
+    if out is None:
+        out = torch.zeros(q8.shape, dtype=_I8, device=q8.device)
+    code = _calls.attention(_attention_at, q8, k_pages, v_pages, table, length, q_start, score_rq, out_rq, prob_bits, max_rows, max_len,
+                            seqs, out, status)
+    if code is None:  # something unusual, or wrong
+        code = _attention_checked(q8, k_pages, v_pages, table, length, q_start, score_rq, out_rq, prob_bits, max_rows, max_len, seqs,
+                                  out, status)
+    if code:
+        _check_code(lib, code)
+    return out
+
+
+def _attention_checked(q8, k_pages, v_pages, table, length, q_start, score_rq, out_rq, prob_bits, max_rows, max_len, seqs, out,
+                       status) -> int:
     dev = _cuda(q8, "q8")
-    if (not (q8.dtype is k_pages.dtype is v_pages.dtype is _I8) or not (table.dtype is length.dtype is q_start.dtype is _I32)
-            or not (dev == k_pages.get_device() == v_pages.get_device() == table.get_device() == length.get_device()
-                    == q_start.get_device()) or out is not None or seqs is not None or status is not None):
-        _refuse(dev, _I8, q8=q8, k_pages=k_pages, v_pages=v_pages, out=out)
-        _refuse(dev, _I32, table=table, length=length, q_start=q_start, seqs=seqs, status=status)
+    _refuse(dev, _I8, q8=q8, k_pages=k_pages, v_pages=v_pages, out=out)
+    _refuse(dev, _I32, table=table, length=length, q_start=q_start, seqs=seqs, status=status)
     if len(q8.shape) != 3 or len(k_pages.shape) != 4:
         raise ValueError("q8 must be [rows, n_heads, head_dim], k_pages [n_pages, n_kv_heads, page_size, head_dim]")
     R, H, D = q8.shape
     _, page_stride, _, n_pages, Hkv, P, Dk = _pool(k_pages, v_pages)
     if D != Dk:
         raise ValueError(f"q8 has heads of {D}, the cache of {Dk}")
-    if out is None:
-        out = torch.zeros((R, H, D), dtype=_I8, device=k_pages.device)
     starts, slots, n = _launch(q_start, seqs)
     _need_slots(seqs, n, table)
     args = _ATTENTION.pack(q8.data_ptr(), out.data_ptr(), _rows(q8, "q8", H, D, R), _rows(out, "out", H, D, R), R, H, Hkv, D,
                            k_pages.data_ptr(), v_pages.data_ptr(), page_stride, n_pages, P, *_table(table, length),
                            length.data_ptr(), starts, slots, n, max_rows, max_len, *score_rq, *out_rq, prob_bits,
                            status.data_ptr() if status is not None else 0, dev)
-    lib = _lib or _load()
-    code = lib.llx_paged_attention(args, _stream(dev))
-    if code:
-        _check_code(lib, code)
-    return out
+    return (_lib or _load()).llx_paged_attention(args, _stream(dev))
 
 
 def _page_call(name, pool, table, length, refs, list_a, list_b, share, new_table, new_refs, status) -> None:

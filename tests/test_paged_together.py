@@ -239,3 +239,32 @@ def test_chunk_over_a_long_context():
         PO.attention(q, k, v, *args, rq, (1717986918, 36), 15, None, 10, T, want)
         got = paged.attention(dev(q), dev(k), dev(v), *map(dev, args), rq, (1717986918, 36), max_rows=10, max_len=T)
         assert np.array_equal(got.cpu().numpy(), want)
+
+
+def test_numbers_of_other_types_and_refusals():
+    """numpy numbers and lists are looked at in Python: the same results, and the same words for what is wrong."""
+    s = Steps(np.random.default_rng(1), 4, 2, 64, 16, 2, 4)
+    x, t = s.inputs([9, 1], [0, 1])
+    paged.reserve(s.table, s.length, s.refs, t["slots"], t["counts"], 16, status=s.t["st"])
+    args = [t["q"], t["k"], t["v"], s.tk, s.tv, s.table, s.length, t["q_start"], s.t["cos"], s.t["sin"]]
+    norm = (s.t["norm"][0], *(np.int64(n) for n in s.t["norm"][1:]))
+    q8 = [paged.append(*args, Q_RQ, K_RQ, q_norm=s.t["norm"], k_norm=s.t["norm"], seqs=t["slots"], status=s.t["st"]),
+          paged.append(*args, list(Q_RQ), np.array(K_RQ), q_norm=norm, k_norm=list(norm), seqs=t["slots"])]
+    assert torch.equal(*q8) and int(q8[0].abs().max()) > 0
+    args = [q8[0], s.tk, s.tv, s.table, s.length, t["q_start"]]
+    o = [paged.attention(*args, SCORE, OUT, max_rows=9, max_len=64, seqs=t["slots"], status=s.t["st"]),
+         paged.attention(*args, list(SCORE), np.array(OUT), prob_bits=np.int32(15), max_rows=np.int64(9), max_len=np.int64(64),
+                         seqs=t["slots"])]
+    assert torch.equal(*o) and int(o[0].abs().max()) > 0
+    for i, wrong, words in ((0, q8[0].short(), "q8 must be torch.int8"), (1, s.tk[:, :, :8], "alike"), (2, s.tv.cpu(), "must be on cuda"),
+                            (3, s.table.t(), "dense rows"), (4, s.length[:1], "entry per slot"), (5, t["q_start"][::2], "dense vector"),
+                            (0, q8[0][..., ::2], "heads of 32"), (0, q8[0].transpose(0, 1), "must be|dense")):
+        bad = list(args)
+        bad[i] = wrong
+        with pytest.raises(ValueError, match=words):
+            paged.attention(*bad, SCORE, OUT, max_rows=9, max_len=64, seqs=t["slots"], out=torch.zeros_like(q8[0]))
+    with pytest.raises(ValueError, match="prob_bits"):
+        paged.attention(*args, SCORE, OUT, prob_bits=9, max_rows=9, max_len=64, seqs=t["slots"])
+    with pytest.raises(ValueError, match="outside M"):
+        paged.attention(*args, (-1, 3), OUT, max_rows=9, max_len=64, seqs=t["slots"])
+    assert int(s.t["st"].item()) == 0
