@@ -202,7 +202,8 @@ llx_status llx_linear_argmax_noalloc(const int8_t* A, const int8_t* W, const int
  * of every query and key head (gamma null: none), rotation (cos / sin [n_positions][head_dim / 2]
  * Q1.14), requantization to i8 (M, S); q8 [rows][n_heads][head_dim] is written, keys and values
  * go to their pages.  Strides are in elements between rows. A row without a place in the cache
- * (see status) gets zeros in q8 and writes no page. */
+ * (see status) gets zeros in q8 and writes no page.  A slot may be listed once in seqs: its rows are
+ * its newest positions. */
 typedef struct {
   const int16_t *q, *k;
   const int8_t* v;

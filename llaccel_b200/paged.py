@@ -150,7 +150,7 @@ def append(q, k, v, k_pages, v_pages, table, length, q_start, cos, sin, q_rq, k_
     query and key head an RMSNorm (`q_norm` / `k_norm` = (gamma int16 [head_dim], eps_t, C,
     sh_post), or None), the rotation at the row's position (`cos`, `sin` int16 Q1.14
     [positions, head_dim / 2]) and requantization by `q_rq` / `k_rq` = (M, S).  Keys and values go
-    to the pages of their positions.  Returns the int8 queries, in `out` if given; rows behind
+    to the pages of their positions; a slot may be listed once.  Returns the int8 queries, in `out` if given; rows behind
     `q_start[-1]` are left as they were."""
     lib = _lib or _load()
     if out is None:
