@@ -105,9 +105,10 @@ __global__ void __launch_bounds__(256) k_paged_append_any(const llx_paged_append
 // head, each with 8 neighbouring values and their 8 partners half a head away: one 16-byte load each,
 // and a rotation without exchange.  The row's place is looked up while those loads are under way.
 // Per row 2 (H + Hkv) D + Hkv D bytes read, H D + 2 Hkv D written.  8,000 rows of 16 + 8 heads of 128 with
-// norms: 92 MB in 40 us, 2.3 TB/s; its instructions bound it (65 % of the issue slots; 64-bit products of
-// norm and requantization, some 42 instructions a value), the copy rate would allow 14 us.  A block per
-// row and a warp per head with single loads took 166.  A single row takes 3.2 us inside a graph, most of it latency.
+// norms: 92 MB in 38 us, 2.4 TB/s; its instructions bound it (65 % of the issue slots; 64-bit products of
+// norm and requantization, some 40 instructions a value), the copy rate would allow 14 us.  A block per
+// row and a warp per head with single loads took 166; one lane per head for square root and quotient, after
+// a first reading of the row, 47.  A single row takes 3.2 us inside a graph, most of it latency.
 struct AppendSide {
   const int16_t *x, *gamma;
   int64_t eps, C, stride;
@@ -231,9 +232,10 @@ __global__ void __launch_bounds__(128) k_paged_append(const llx_paged_append_arg
     int z1[8], z2[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      // of 16-bit values x1 c - x2 s stays in 32 bits with the rounding; x2 c + x1 s can be 2^31
+      // of 16-bit values x1 c - x2 s stays in 32 bits with the rounding; x2 c + x1 s can be 2^31, but not
+      // with 2^14 less (and is -2^31 + 2^16 at least), which its quotient gets back as 1
       const int y1 = __viaddmin_s32_relu((x1[j] * c[j] - x2[j] * n[j] + 8192) >> 14, 32768, 65535);
-      const int y2 = __viaddmin_s32_relu((int)(((int64_t)x2[j] * c[j] + (int64_t)x1[j] * n[j] + 8192) >> 14), 32768, 65535);
+      const int y2 = __viaddmin_s32_relu((x2[j] * c[j] - 8192 + x1[j] * n[j]) >> 14, 32769, 65535);
       z1[j] = (int)(((int64_t)y1 * s.M + half) >> 32) >> sh;
       z2[j] = (int)(((int64_t)y2 * s.M + half) >> 32) >> sh;
     }

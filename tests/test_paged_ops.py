@@ -100,6 +100,26 @@ def test_append_one_norm_only_and_extremes():
     assert append_case(rng, 4, 4, 128, 64, [5], [70], True, sd=30000.0, edit=edit) == 0
 
 
+@pytest.mark.parametrize("D", [16, 64, 128, 48])
+def test_append_rotation_at_the_ends_of_16_bits(D):
+    """x2 c + x1 s from -2^31 + 2^16 to 2^31, which 32 bits hold only one by one."""
+    H, Hkv, P, ends = 4, 2, 16, np.array([-32768, 32767], np.int16)
+    rng = np.random.default_rng(D)
+    L = launch(rng, [64], [64], P)
+    q, k = (rng.choice(ends, (64, h, D)) for h in (H, Hkv))
+    v = np.zeros((64, Hkv, D), np.int8)
+    cos, sin = (rng.choice(ends, (64, D // 2)) for _ in "cs")
+    rq = (1142505715, 38)
+    want = [np.zeros((64, H, D), np.int8)] + [np.zeros((L["N"], Hkv, P, D), np.int8) for _ in "kv"]
+    got = [dev(w) for w in want]
+    PO.append(q, k, v, want[1], want[2], L["table"], L["length"], L["q_start"], cos, sin, rq, rq, None, None, None, want[0])
+    paged.append(dev(q), dev(k), dev(v), got[1], got[2], dev(L["table"]), dev(L["length"]), dev(L["q_start"]), dev(cos), dev(sin), rq,
+                 rq, out=got[0])
+    for g, w in zip(got, want):
+        assert np.array_equal(g.cpu().numpy(), w)
+    assert len(np.unique(want[0])) > 2
+
+
 def test_append_skips_rows_without_a_place():
     rng = np.random.default_rng(3)
 
