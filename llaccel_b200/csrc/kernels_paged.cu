@@ -127,16 +127,18 @@ __device__ __forceinline__ void unpack8(const uint4& v, int (&x)[8]) {
 }
 __device__ __forceinline__ int clamp32(int v, int lo, int hi) { return max(lo, min(hi, v)); }
 
-// floor(sqrt(t)) for t < 2^48: a float root is off by less than 2, integer products settle it
+// floor(sqrt(t)) for t < 2^48: an approximate root is off by a few at most, integer products settle it
 __device__ __forceinline__ uint32_t root48(uint64_t t) {
-  uint32_t r = (uint32_t)sqrtf((float)t);
+  float f;
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(f) : "f"((float)t));
+  uint32_t r = (uint32_t)f;
   while ((uint64_t)r * r > t) --r;
   while ((uint64_t)(r + 1) * (r + 1) <= t) ++r;
   return r;
 }
-// min(65535, C / r) for C < 2^40, 1 <= r < 2^24: below 2^17 a float quotient is off by less than 1
+// min(65535, C / r) for C < 2^40, 1 <= r < 2^24: below 2^17 an approximate quotient (2 ulp) is off by less than 1
 __device__ __forceinline__ uint32_t inverse16(uint64_t C, uint32_t r) {
-  const float f = (float)C / (float)r;
+  const float f = __fdividef((float)C, (float)r);
   uint32_t q = f >= 65536.0f ? 65536u : (uint32_t)f;
   while ((uint64_t)q * r > C) --q;
   while (q < 65536u && (uint64_t)(q + 1) * r <= C) ++q;
