@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(256) k_paged_append_any(const llx_paged_append
 // head, each with 8 neighbouring values and their 8 partners half a head away: one 16-byte load each,
 // and a rotation without exchange.  The row's place is looked up while those loads are under way.
 // Per row 2 (H + Hkv) D + Hkv D bytes read, H D + 2 Hkv D written.  8,000 rows of 16 + 8 heads of 128 with
-// norms: 92 MB in 38 us, 2.4 TB/s; its instructions bound it (65 % of the issue slots; 64-bit products of
+// norms: 92 MB in 37 us, 2.5 TB/s; its instructions bound it (65 % of the issue slots; 64-bit products of
 // norm and requantization, some 40 instructions a value), the copy rate would allow 14 us.  A block per
 // row and a warp per head with single loads took 166; one lane per head for square root and quotient, after
 // a first reading of the row, 47.  A single row takes 3.2 us inside a graph, most of it latency.
@@ -212,7 +212,7 @@ __global__ void __launch_bounds__(128) k_paged_append(const llx_paged_append_arg
     if (s.gamma) {
       uint64_t ss = 0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) ss += (uint64_t)((int64_t)x1[j] * x1[j]) + (uint64_t)((int64_t)x2[j] * x2[j]);
+      for (int j = 0; j < 8; ++j) ss += (uint32_t)(x1[j] * x1[j]) + (uint32_t)(x2[j] * x2[j]);  // 2^31 at most
 #pragma unroll
       for (int o = 1; o < L; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
       const uint32_t root = root48(ss + (uint64_t)s.eps);
