@@ -20,6 +20,8 @@
 // 2,100 to 4,000 earlier keys, 32 heads on 8: 273 us, 0.35 PFLOP/s of the operator's own products.  Steps:
 // one block per row and head 57,717 us; this form 494; exponentials from one table 405; whole tiles without
 // masks and cheaper waits 372; the table in words 323; page ids read ahead 303; a second loading warp 273.
+// A tile's keys stay with one CTA: launches of few tiles over long contexts leave SMs idle (14 CTAs for 110
+// rows, 16 heads on 2, about 50k keys: 1.1 ms).
 // Roles: warps 0 and 1 load (every other stage), warps 2 and 3 issue the MMAs (every other score tile of
 // passes 1 and 2; the scores and the values of pass 3), warps 4 to 19 do the softmax.
 #include <atomic>
