@@ -298,24 +298,25 @@ cudaError_t launch_paged_append(const llx_paged_append_args& a, cudaStream_t st)
 constexpr int kPlanThreads = 1024;
 constexpr int kMaxSlots = 1 << 18;  // slots of a table (bitmap of 32 KB)
 
-// exclusive sum over the block; *total gets the whole
-__device__ int block_scan(int v, int* total) {
-  __shared__ int part[kPlanThreads / 32];
+// exclusive sum over the block; *total gets the whole.  In 64 bits: a slot may ask for 2^24 pages, so the
+// threads of one round for 2^34, and a request must not wrap into one that can be met.
+__device__ int64_t block_scan(int64_t v, int64_t* total) {
+  __shared__ int64_t part[kPlanThreads / 32];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  int x = v;
+  int64_t x = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
     if (lane >= o) x += y;
   }
   __syncthreads();  // part may still be read by an earlier call
   if (lane == 31) part[w] = x;
   __syncthreads();
   if (w == 0) {
-    int y = part[lane];
+    int64_t y = part[lane];
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int z = __shfl_up_sync(0xffffffffu, y, o);
+      const int64_t z = __shfl_up_sync(0xffffffffu, y, o);
       if (lane >= o) y += z;
     }
     part[lane] = y;
@@ -372,9 +373,9 @@ __device__ void count_pages(const llx_pages_args& a, const int32_t* slots, int s
 __device__ bool take_free(const llx_pages_args& a, int64_t need) {
   const int64_t per = (a.n_pages + kPlanThreads - 1) / kPlanThreads;
   const int64_t p0 = threadIdx.x * per, p1 = p0 + per < a.n_pages ? p0 + per : a.n_pages;
-  int mine = 0, have;
+  int64_t mine = 0, have;
   for (int64_t p = p0; p < p1; ++p) mine += a.refs[p] <= 0;
-  int at = block_scan(mine, &have);
+  int64_t at = block_scan(mine, &have);
   if (have < need) return false;
   for (int64_t p = p0; p < p1 && at < need; ++p)
     if (a.refs[p] <= 0) a.scratch[at++] = (int32_t)p;
@@ -396,14 +397,14 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_reserve(const llx_pages_
   int64_t need = 0;
   for (int64_t i0 = 0; i0 < a.n; i0 += kPlanThreads) {
     const int64_t i = i0 + threadIdx.x;
-    int mine = 0, sum;
+    int64_t mine = 0, sum;
     if (i < a.n) {
       const int s = a.list_a[i];
       const int64_t len = a.length[s], more = a.list_b[i];
       if (len < 0 || more < 0 || len + more > a.max_pages * P) {
         atomicOr(&code, LLX_STATUS_BAD_POSITION);
       } else {
-        mine = (int)(pages_for(len + more, P) - pages_for(len, P));
+        mine = pages_for(len + more, P) - pages_for(len, P);
         if (more && len % P) {
           const int id = a.table[s * a.table_stride + len / P];
           if (id < 0 || id >= a.n_pages) atomicOr(&code, LLX_STATUS_BAD_PAGE);
@@ -422,15 +423,15 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_reserve(const llx_pages_
   int64_t base = 0;
   for (int64_t i0 = 0; i0 < a.n; i0 += kPlanThreads) {
     const int64_t i = i0 + threadIdx.x;
-    int s = 0, mine = 0, sum;
-    int64_t len = 0;
+    int s = 0;
+    int64_t len = 0, mine = 0, sum;
     if (i < a.n) {
       s = a.list_a[i];
       len = a.length[s];
-      mine = (int)(pages_for(len + a.list_b[i], P) - pages_for(len, P));
+      mine = pages_for(len + a.list_b[i], P) - pages_for(len, P);
     }
     const int64_t at = base + block_scan(mine, &sum);
-    for (int j = 0; j < mine; ++j) {
+    for (int64_t j = 0; j < mine; ++j) {
       const int id = a.scratch[at + j];
       a.table[s * a.table_stride + pages_for(len, P) + j] = id;
       a.refs[id] = 1;
@@ -477,10 +478,10 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_fork(const llx_pages_arg
   int64_t need = 0;
   for (int64_t i0 = 0; i0 < a.n; i0 += kPlanThreads) {
     const int64_t i = i0 + threadIdx.x;
-    int mine = 0, sum;
+    int64_t mine = 0, sum;
     if (i < a.n) {
       const int64_t len = slot_length(a, a.list_a[i]);
-      mine = (int)(pages_for(len, P) - (a.share ? len / P : 0));
+      mine = pages_for(len, P) - (a.share ? len / P : 0);
     }
     block_scan(mine, &sum);
     need += sum;
@@ -498,12 +499,12 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_fork(const llx_pages_arg
   int64_t base = 0;
   for (int64_t i0 = 0; i0 < a.n; i0 += kPlanThreads) {
     const int64_t i = i0 + threadIdx.x;
-    int mine = 0, sum;
+    int64_t mine = 0, sum;
     if (i < a.n) {
       const int64_t len = slot_length(a, a.list_a[i]);
-      mine = (int)(pages_for(len, P) - (a.share ? len / P : 0));
+      mine = pages_for(len, P) - (a.share ? len / P : 0);
     }
-    first[threadIdx.x] = block_scan(mine, &sum);
+    first[threadIdx.x] = (int)block_scan(mine, &sum);  // below `need`, which is at most n_pages
     __syncthreads();
     for (int64_t x = warp; x < kPlanThreads && i0 + x < a.n; x += kPlanThreads / 32) {
       const int from = a.list_a[i0 + x], to = a.list_b[i0 + x];
@@ -589,9 +590,10 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_compact(const llx_pages_
   const int64_t N = a.n_pages, per = (N + kPlanThreads - 1) / kPlanThreads;
   const int64_t p0 = min(N, threadIdx.x * per), p1 = min(N, p0 + per);
   int32_t *to = a.scratch, *src = to + N, *dst = src + N;
-  int used = 0, live, moves;
+  int64_t used = 0, all;
   for (int64_t p = p0; p < p1; ++p) used += a.refs[p] > 0;
-  const int before = block_scan(used, &live);  // live pages below p0
+  const int before = (int)block_scan(used, &all);  // live pages below p0
+  const int live = (int)all;
   // movers: live pages from id `live` on; holes: free pages below it; as many of each.  Of the pages
   // below `live`, those that are not live are holes; of the live pages, those past the ones below it move.
   __shared__ int live_below;  // live pages with an id below `live`
@@ -601,7 +603,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_compact(const llx_pages_
     live_below = n;
   }
   __syncthreads();
-  moves = live - live_below;
+  const int moves = live - live_below;
   int n = before;
   for (int64_t p = p0; p < p1; ++p) {
     const bool l = a.refs[p] > 0;

@@ -1,0 +1,53 @@
+"""The paged-serving calls at the ends of what their arguments can say."""
+from __future__ import annotations
+
+import subprocess
+
+import numpy as np
+import pytest
+
+from conftest import REPO
+
+torch = pytest.importorskip("torch")
+
+gpu = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def paged():
+    from llaccel_b200 import build
+    build.build()
+    from llaccel_b200 import paged
+    return paged
+
+
+def ints(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def test_page_counts_add_up_in_64_bits(tmp_path):
+    from llaccel_b200 import build as B
+    r = subprocess.run([B.nvcc(), "-std=c++17", *B.ARCH_FLAGS, "--expt-relaxed-constexpr", "-I", str(B.INCLUDE), "-I", str(B.CSRC), "-c",
+                        str(REPO / "tests" / "paged_plan_check.cu"), "-o", str(tmp_path / "check.o")], capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr[-3000:]
+
+
+@gpu
+def test_requests_beyond_32_bits_of_pages_are_refused(paged):
+    """128 slots of 2^24 pages each: 2^31 pages, of a cache that has four."""
+    W, P, N = 1 << 24, 16, 4
+    if torch.cuda.mem_get_info()[0] < 16 << 30:
+        pytest.skip("needs a page table of 8 GB")
+    table = torch.full((129, W), -1, dtype=torch.int32, device="cuda")
+    length, refs = torch.zeros(129, dtype=torch.int32, device="cuda"), ints([0, 1, 0, 0])
+    status = ints([0])
+    paged.reserve(table, length, refs, ints(range(1, 129)), torch.full((128,), W * P, dtype=torch.int32, device="cuda"), P, status=status)
+    assert int(status.item()) == 8
+    assert not length.any() and refs.tolist() == [0, 1, 0, 0] and int(table.max()) == -1
+    status.zero_()
+    length[0] = W * P
+    k, v = (torch.zeros((N, 1, P, 16), dtype=torch.int8, device="cuda") for _ in "kv")
+    paged.fork(k, v, table, length, refs, torch.zeros(128, dtype=torch.int32, device="cuda"), ints(range(1, 129)), share=False,
+               status=status)
+    assert int(status.item()) == 8
+    assert not length[1:].any() and refs.tolist() == [0, 1, 0, 0] and int(table.max()) == -1
