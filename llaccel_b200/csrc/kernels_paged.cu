@@ -474,7 +474,15 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_fork(const llx_pages_arg
     return;
   }
   const int64_t P = a.page_size;
-  count_pages(a, a.list_b, -1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // what is to be copied has to be there, before anything is changed
+  __shared__ int bad;
+  if (threadIdx.x == 0) bad = 0;
+  __syncthreads();
+  auto there = [&](int slot, int64_t j) {
+    const int id = a.table[slot * a.table_stride + j];
+    if (id < 0 || id >= a.n_pages) bad = 1;
+  };
   int64_t need = 0;
   for (int64_t i0 = 0; i0 < a.n; i0 += kPlanThreads) {
     const int64_t i = i0 + threadIdx.x;
@@ -482,10 +490,25 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_fork(const llx_pages_arg
     if (i < a.n) {
       const int64_t len = slot_length(a, a.list_a[i]);
       mine = pages_for(len, P) - (a.share ? len / P : 0);
+      if (a.share && mine) there(a.list_a[i], len / P);
     }
     block_scan(mine, &sum);
     need += sum;
   }
+  if (!a.share)
+    for (int64_t i = warp; i < a.n; i += kPlanThreads / 32) {
+      const int64_t held = pages_for(slot_length(a, a.list_a[i]), P);
+      for (int64_t j = lane; j < held; j += 32) there(a.list_a[i], j);
+    }
+  __syncthreads();
+  if (bad) {
+    if (threadIdx.x == 0) {
+      raise_status(a.status, LLX_STATUS_BAD_PAGE);
+      *done = 0;
+    }
+    return;
+  }
+  count_pages(a, a.list_b, -1);
   if (!take_free(a, need)) {
     count_pages(a, a.list_b, 1);
     if (threadIdx.x == 0) {
@@ -494,7 +517,6 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_fork(const llx_pages_arg
     }
     return;
   }
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   __shared__ int first[kPlanThreads];
   int64_t base = 0;
   for (int64_t i0 = 0; i0 < a.n; i0 += kPlanThreads) {

@@ -115,6 +115,10 @@ class Pages:
         if not self._slots_fine(children, parents):
             return 16, []
         P, keep = self.P, self.refs.copy()
+        for p in parents:  # what is to be copied has to be there
+            n = max(0, min(int(self.length[p]), self.table.shape[1] * P))
+            if any(not 0 <= self.table[p][j] < len(keep) for j in range(n // P if share else 0, -(-n // P))):
+                return 1, []
         for c in children:
             self._release(c)
         free = np.flatnonzero(self.refs <= 0)

@@ -45,9 +45,29 @@ def test_requests_beyond_32_bits_of_pages_are_refused(paged):
     assert int(status.item()) == 8
     assert not length.any() and refs.tolist() == [0, 1, 0, 0] and int(table.max()) == -1
     status.zero_()
-    length[0] = W * P
+    length[0], table[0] = W * P, 1
     k, v = (torch.zeros((N, 1, P, 16), dtype=torch.int8, device="cuda") for _ in "kv")
     paged.fork(k, v, table, length, refs, torch.zeros(128, dtype=torch.int32, device="cuda"), ints(range(1, 129)), share=False,
                status=status)
     assert int(status.item()) == 8
-    assert not length[1:].any() and refs.tolist() == [0, 1, 0, 0] and int(table.max()) == -1
+    assert not length[1:].any() and refs.tolist() == [0, 1, 0, 0] and int(table[1:].max()) == -1
+
+
+@gpu
+@pytest.mark.parametrize("share", [True, False])
+@pytest.mark.parametrize("bad", [-1, 9, 1 << 30])
+def test_a_fork_of_a_page_that_is_not_there_changes_nothing(paged, share, bad):
+    """Among good pairs; the page of the copy used to be some former owner's."""
+    rng = np.random.default_rng(0)
+    N, P, status = 9, 16, ints([0])
+    k, v = (torch.from_numpy(rng.integers(-128, 128, (2, N, 2, P, 32)).astype(np.int8)).cuda() for _ in "kv")
+    table = ints([[4, 0, -1], [7, -1, -1], [bad if not share else 5, bad if share else 6, -1], [2, 8, -1], [-1] * 3])
+    length, refs = ints([20, 16, 20, 30, 0]), ints([1, 0, 1, 0, 1, 1, 1, 1, 1])
+    before = [t.clone() for t in (k, v, table, length, refs)]
+    paged.fork(k, v, table, length, refs, ints([0, 2]), ints([3, 4]), share=share, status=status)
+    assert int(status.item()) == 1
+    assert all(torch.equal(x, y) for x, y in zip(before, (k, v, table, length, refs)))
+    paged.fork(k, v, table, length, refs, ints([0, 1]), ints([3, 4]), share=share, status=status.zero_())
+    assert int(status.item()) == 0 and length.tolist() == [20, 16, 20, 20, 16]
+    new = table[3, 1].long()
+    assert torch.equal(k[:, new, :, :4], before[0][:, 0, :, :4])
