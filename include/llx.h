@@ -308,7 +308,12 @@ llx_status llx_sample(const llx_sample_args* a, void* stream);
  * rows are sampled.  Results are those of llx_generate on each sequence alone, bit for bit.
  * max_seqs slots share n_pages pages of page_size positions; a step has max_rows tokens at most.
  * One GPU, graphs of the fused op list (llx_opts.fuse = 1).  Not thread-safe; every call waits for
- * its work. */
+ * its work.
+ * LLX_ERR_OOM means that nothing was changed.  Another failure (LLX_ERR_CUDA, LLX_ERR_DEVICE) may come
+ * when a step's pages are taken and some layers' keys are not written: its slots (a fork's children)
+ * are then refused with LLX_ERR_INVALID until they are freed; a child of another fork is as good as
+ * freed.  The other slots go on.  After a compaction that failed every call but usage and destroy
+ * is refused. */
 typedef struct llx_serve llx_serve;
 /* per sequence of a step (each array may be null, see llx_sample); random null: largest logit */
 typedef struct {

@@ -861,6 +861,8 @@ struct PagedState {
   double* random = nullptr;
   std::vector<void*> owned;
   std::vector<int> len;             // host copy of the lengths
+  std::vector<char> broken;         // slots that a failed call left half done: closed until they are freed
+  bool damaged = false;             // a compaction failed half way: the tables are of no more use
   std::vector<int> q_norm, k_norm;  // per plan step: the norm steps its append takes over, or -1
   std::vector<char> skipped;        // per plan step: a norm that an append takes over
   int n = 0, rows = 0, max_rows = 0, max_len = 0;  // the launch under way
@@ -1890,6 +1892,7 @@ static void paged_create(llx_model* m, int max_seqs, int n_pages, int page_size,
   p.top_k = paged_alloc<int32_t>(p, max_seqs);
   p.random = paged_alloc<double>(p, max_seqs);
   p.len.assign(max_seqs, 0);
+  p.broken.assign(max_seqs, 0);
   LLX_CUDA(cudaDeviceSynchronize());
 }
 
@@ -1923,16 +1926,32 @@ static llx_pages_args paged_pages(llx_session* s, int n) {
   return a;
 }
 
-// waits for the stream; what the device found wrong since the last call becomes an error
-static void paged_check(llx_session* s) {
+// waits for the stream; what the device found wrong since the last call
+static int32_t paged_status(llx_session* s) {
   PagedState& p = *s->paged;
   int32_t code = 0;
   LLX_CUDA(cudaMemcpyAsync(&code, p.status, sizeof(code), cudaMemcpyDeviceToHost, s->st));
   LLX_CUDA(cudaStreamSynchronize(s->st));
-  if (!code) return;
-  LLX_CUDA(cudaMemsetAsync(p.status, 0, sizeof(code), s->st));
-  require(!(code & LLX_STATUS_NO_PAGES), LLX_ERR_OOM, "the cache has too few free pages");
-  throw Error(LLX_ERR_DEVICE, "a paged call found its tables damaged (status " + std::to_string(code) + ")");
+  if (code) LLX_CUDA(cudaMemsetAsync(p.status, 0, sizeof(code), s->st));
+  return code;
+}
+
+static void paged_accept(int32_t code) {
+  require(!code, LLX_ERR_DEVICE, "a paged call found its tables damaged (status " + std::to_string(code) + ")");
+}
+
+// What a call does once it has begun to change slots.  LLX_ERR_OOM tells the caller that nothing was changed,
+// so it is not among the errors that come out of here.
+template <class F>
+static void paged_commit(F&& f) {
+  try {
+    f();
+  } catch (const Error& e) {
+    if (e.code == LLX_ERR_OOM) throw Error(LLX_ERR_CUDA, e.what());
+    throw;
+  } catch (const std::bad_alloc&) {
+    throw Error(LLX_ERR_CUDA, "host allocation failed");
+  }
 }
 
 static int paged_need(const PagedState& p, int len) { return (len + p.page_size - 1) / p.page_size; }
@@ -1945,6 +1964,7 @@ static int64_t paged_free_at_least(const PagedState& p) {
 }
 
 static void paged_slots(const PagedState& p, int n, const int32_t* slots, bool once) {
+  require(!p.damaged, LLX_ERR_INVALID, "a compaction of this cache failed half way: destroy it");
   require(n >= 0 && n <= p.max_seqs && (n == 0 || slots), LLX_ERR_INVALID, "a list of at most max_seqs slots");
   std::vector<char> seen(once ? p.max_seqs : 0, 0);
   for (int i = 0; i < n; ++i) {
@@ -1953,6 +1973,16 @@ static void paged_slots(const PagedState& p, int n, const int32_t* slots, bool o
     require(!seen[slots[i]], LLX_ERR_INVALID, "slot " + std::to_string(slots[i]) + " is listed twice");
     seen[slots[i]] = 1;
   }
+}
+
+static void paged_whole(const PagedState& p, int n, const int32_t* slots) {
+  for (int i = 0; i < n; ++i)
+    require(!p.broken[slots[i]], LLX_ERR_INVALID,
+            "slot " + std::to_string(slots[i]) + " was left half done by a call that failed: free it first");
+}
+
+static void paged_mark(PagedState& p, int n, const int32_t* slots, bool broken) {
+  for (int i = 0; i < n; ++i) p.broken[slots[i]] = broken;
 }
 
 }  // namespace llx
@@ -2495,6 +2525,7 @@ llx_status llx_serve_step(llx_serve* h, int n, const int32_t* slots, const int32
     PagedState& p = *s->paged;
     require(n >= 1, LLX_ERR_INVALID, "a step needs a sequence");
     paged_slots(p, n, slots, true);
+    paged_whole(p, n, slots);
     std::vector<int32_t> starts(n + 1, 0), last(n);
     int64_t rows = 0, pages = 0;
     int most = 0, longest = 0;
@@ -2517,59 +2548,74 @@ llx_status llx_serve_step(llx_serve* h, int n, const int32_t* slots, const int32
     const bool sampled = how && how->random;
     require(!sampled || m->vocab <= sample_max_vocab(), LLX_ERR_UNSUPPORTED, "the vocabulary is too large to sample from");
     cudaSetDevice(m->device);
+    if (logits) ensure_i16(s, (size_t)n * m->vocab_padded);
     stage_tokens(s, tokens, (int)rows);
     paged_put(s, p.slots, slots, n);
     paged_put(s, p.counts, counts, n);
     paged_put(s, p.starts, starts.data(), n + 1);
     std::memcpy(s->h_rec, last.data(), sizeof(int32_t) * n);
     LLX_CUDA(cudaMemcpyAsync(s->d_rec, s->h_rec, sizeof(int32_t) * n, cudaMemcpyHostToDevice, s->st));
+    const bool tight = pages > paged_free_at_least(p);
     LLX_CUDA(launch_pages_reserve(paged_pages(s, n), s->st));
-    if (pages > paged_free_at_least(p)) paged_check(s);  // nothing was taken when there were too few
+    paged_mark(p, n, slots, true);  // until the step is done
     for (int i = 0; i < n; ++i) p.len[slots[i]] += counts[i];
-    p.n = n;
-    p.rows = (int)rows;
-    p.max_rows = most;
-    p.max_len = longest;
-    const Binding bd = bind(s, false);
-    enqueue_steps(s, bd, 0, m->tail_start, (int)rows, (int)rows);
-    Binding bt = bd;
-    for (size_t t = 0; t < m->tail_inputs.size(); ++t) {
-      const int a = m->tail_inputs[t];
-      void* dst = s->arena + s->tail_off[t];
-      LLX_CUDA(launch_gather_rows(bd.p[a], dst, s->d_rec, n, m->acts[a].cols * m->acts[a].elem, s->st));
-      bt.p[a] = dst;
-      bt.rows[a] = s->tail_rows_alloc;
-    }
-    enqueue_steps(s, bt, m->tail_start, m->steps.size(), n, n);
-    const int16_t* out = (const int16_t*)bd.p[m->output_act];
-    if (!sampled) {
-      launch_output_argmax(s, out, n);
-    } else {
-      llx_sample_args a{};
-      a.logits = out;
-      a.logits_stride = m->vocab_padded;
-      a.rows = n;
-      a.vocab = m->vocab;
-      a.exponent = m->E_LOGIT;
-      auto put = [&](auto* dst, const auto* src) { paged_put(s, dst, src, src ? n : 0); };
-      put(p.random, how->random);
-      put(p.temperature, how->temperature);
-      put(p.top_k, how->top_k);
-      put(p.top_p, how->top_p);
-      put(p.min_p, how->min_p);
-      a.random = p.random;
-      a.temperature = how->temperature ? p.temperature : nullptr;
-      a.top_k = how->top_k ? p.top_k : nullptr;
-      a.top_p = how->top_p ? p.top_p : nullptr;
-      a.min_p = how->min_p ? p.min_p : nullptr;
-      a.token = s->d_argmax;
-      a.prob = p.prob;
-      LLX_CUDA(launch_sample(a, s->st));
-      if (prob) LLX_CUDA(cudaMemcpyAsync(prob, p.prob, sizeof(float) * n, cudaMemcpyDeviceToHost, s->st));
-    }
-    paged_check(s);
-    check_device_error(s);
-    copy_outputs(s, n, logits, next);
+    bool full = false;
+    paged_commit([&] {
+      if (tight) {
+        const int32_t code = paged_status(s);
+        full = code & LLX_STATUS_NO_PAGES;
+        if (full) return;  // nothing was taken
+        paged_accept(code);
+      }
+      p.n = n;
+      p.rows = (int)rows;
+      p.max_rows = most;
+      p.max_len = longest;
+      const Binding bd = bind(s, false);
+      enqueue_steps(s, bd, 0, m->tail_start, (int)rows, (int)rows);
+      Binding bt = bd;
+      for (size_t t = 0; t < m->tail_inputs.size(); ++t) {
+        const int a = m->tail_inputs[t];
+        void* dst = s->arena + s->tail_off[t];
+        LLX_CUDA(launch_gather_rows(bd.p[a], dst, s->d_rec, n, m->acts[a].cols * m->acts[a].elem, s->st));
+        bt.p[a] = dst;
+        bt.rows[a] = s->tail_rows_alloc;
+      }
+      enqueue_steps(s, bt, m->tail_start, m->steps.size(), n, n);
+      const int16_t* out = (const int16_t*)bd.p[m->output_act];
+      if (!sampled) {
+        launch_output_argmax(s, out, n);
+      } else {
+        llx_sample_args a{};
+        a.logits = out;
+        a.logits_stride = m->vocab_padded;
+        a.rows = n;
+        a.vocab = m->vocab;
+        a.exponent = m->E_LOGIT;
+        auto put = [&](auto* dst, const auto* src) { paged_put(s, dst, src, src ? n : 0); };
+        put(p.random, how->random);
+        put(p.temperature, how->temperature);
+        put(p.top_k, how->top_k);
+        put(p.top_p, how->top_p);
+        put(p.min_p, how->min_p);
+        a.random = p.random;
+        a.temperature = how->temperature ? p.temperature : nullptr;
+        a.top_k = how->top_k ? p.top_k : nullptr;
+        a.top_p = how->top_p ? p.top_p : nullptr;
+        a.min_p = how->min_p ? p.min_p : nullptr;
+        a.token = s->d_argmax;
+        a.prob = p.prob;
+        LLX_CUDA(launch_sample(a, s->st));
+        if (prob) LLX_CUDA(cudaMemcpyAsync(prob, p.prob, sizeof(float) * n, cudaMemcpyDeviceToHost, s->st));
+      }
+      paged_accept(paged_status(s));
+      check_device_error(s);
+      copy_outputs(s, n, logits, next);
+    });
+    paged_mark(p, n, slots, false);
+    if (full)
+      for (int i = 0; i < n; ++i) p.len[slots[i]] -= counts[i];
+    require(!full, LLX_ERR_OOM, "the cache has too few free pages");
   });
 }
 
@@ -2580,23 +2626,33 @@ llx_status llx_serve_fork(llx_serve* h, int n, const int32_t* parents, const int
     PagedState& p = *s->paged;
     paged_slots(p, n, parents, false);
     paged_slots(p, n, children, true);
+    paged_whole(p, n, parents);
     std::vector<char> is_child(p.max_seqs, 0);
     for (int i = 0; i < n; ++i) is_child[children[i]] = 1;
-    int64_t pages = 0;
-    for (int i = 0; i < n; ++i) {
+    for (int i = 0; i < n; ++i)
       require(!is_child[parents[i]], LLX_ERR_INVALID, "slot " + std::to_string(parents[i]) + " is both parent and child");
-      const int len = p.len[parents[i]];
-      pages += paged_need(p, len) - (share ? len / p.page_size : 0);
-    }
     cudaSetDevice(s->m->device);
     paged_put(s, p.slots, parents, n);
     paged_put(s, p.counts, children, n);
     llx_pages_args a = paged_pages(s, n);
     a.share = share != 0;
-    LLX_CUDA(launch_pages_fork(a, s->st));
-    if (pages > paged_free_at_least(p)) paged_check(s);
-    for (int i = 0; i < n; ++i) p.len[children[i]] = p.len[parents[i]];
-    LLX_CUDA(cudaStreamSynchronize(s->st));  // the lists are the caller's
+    const std::vector<char> broken = p.broken;
+    const std::vector<int> len = p.len;
+    paged_mark(p, n, children, true);  // until the call is done
+    for (int i = 0; i < n; ++i) p.len[children[i]] = std::max(len[children[i]], len[parents[i]]);
+    int32_t code = 0;
+    paged_commit([&] {
+      LLX_CUDA(launch_pages_fork(a, s->st));
+      code = paged_status(s);
+    });
+    if (code) {  // nothing was changed
+      p.broken = broken;
+      p.len = len;
+    }
+    require(!(code & LLX_STATUS_NO_PAGES), LLX_ERR_OOM, "the cache has too few free pages");
+    paged_accept(code);
+    paged_mark(p, n, children, false);
+    for (int i = 0; i < n; ++i) p.len[children[i]] = len[parents[i]];
   });
 }
 
@@ -2610,6 +2666,7 @@ llx_status llx_serve_free(llx_serve* h, int n, const int32_t* slots) {
     paged_put(s, p.slots, slots, n);
     LLX_CUDA(launch_pages_free(paged_pages(s, n), s->st));
     for (int i = 0; i < n; ++i) p.len[slots[i]] = 0;
+    paged_mark(p, n, slots, false);
     LLX_CUDA(cudaStreamSynchronize(s->st));
   });
 }
@@ -2619,12 +2676,17 @@ llx_status llx_serve_compact(llx_serve* h) {
     require(h, LLX_ERR_INVALID, "null argument");
     llx_session* s = &h->s;
     PagedState& p = *s->paged;
+    paged_slots(p, 0, nullptr, false);
     cudaSetDevice(s->m->device);
     llx_pages_args a = paged_pages(s, 0);
     a.new_table = p.table;
     a.new_refs = p.refs;
-    LLX_CUDA(launch_pages_compact(a, s->st));
-    LLX_CUDA(cudaStreamSynchronize(s->st));
+    p.damaged = true;  // until the call is done
+    paged_commit([&] {
+      LLX_CUDA(launch_pages_compact(a, s->st));
+      LLX_CUDA(cudaStreamSynchronize(s->st));
+    });
+    p.damaged = false;
   });
 }
 

@@ -499,7 +499,8 @@ class CudaServe:
     `step` takes any number of new tokens per sequence and returns one next token each; `fork` lets
     several answers go on from one prompt, `free` gives a slot back.  Tokens and logits are those of
     CudaModel on each sequence alone, whatever else is in the step.  Too few free pages raise
-    LlxError with code LLX_ERR_OOM and change nothing."""
+    LlxError with code LLX_ERR_OOM and change nothing.  A step that fails otherwise may leave its
+    slots half done: they raise ValueError until they are freed, the others go on."""
 
     def __init__(self, model: CudaModel, *, max_seqs: int, n_pages: int, page_size: int = 64, max_rows: int = 1024) -> None:
         self.model, self.lib = model, model.lib
