@@ -71,6 +71,7 @@ typedef struct {
 /* Load qgraph_dir/{qgraph.json, <weights_file>}, validate every op, upload weights,
  * requant tables, RoPE tables and LUTs to the device. opts may be NULL (defaults). */
 llx_status llx_model_load(const char* qgraph_dir, const llx_opts* opts, llx_model** out);
+/* after the sessions and serving handles made from it */
 void llx_model_destroy(llx_model* m);
 llx_status llx_model_get_info(const llx_model* m, llx_model_info* out);
 

@@ -17,6 +17,7 @@ import ctypes as C
 import json
 import math
 import os
+import weakref
 from pathlib import Path
 
 import numpy as np
@@ -160,7 +161,11 @@ class CudaModel:
         self.dir = Path(qgraph_dir)
         self.batch = int(batch)
         self._owns_model = share is None
+        # what uses the weights that this object or `share` owns: closed before the weights are freed
+        self._users = weakref.WeakSet() if share is None else share._users
         if share is not None:
+            if not share._model:
+                raise ValueError("the model is closed")
             self._model = share._model
             self._shared_from = share  # keeps the owner alive
         else:
@@ -186,6 +191,8 @@ class CudaModel:
         self.E_RES, self.E_LOGIT = info.E_RES, info.E_LOGIT
         self.max_rows = int(max_rows or self.max_seq)
         self.keep_acts = bool(keep_acts)
+        if share is not None:
+            self._users.add(self)
         self._sess = C.c_void_p()
         _check(self.lib, self.lib.llx_session_create(self._model, self.batch, self.max_rows, 1 if keep_acts else 0,
                                                      C.byref(self._sess)))
@@ -195,6 +202,11 @@ class CudaModel:
 
     # ---- lifetime ---------------------------------------------------------------------------
     def close(self) -> None:
+        """Frees the session and, with the object that loaded them, the weights; sessions of
+        `share` and CudaServe objects that use these weights are closed first."""
+        if getattr(self, "_owns_model", False):
+            for user in list(self._users):
+                user.close()
         if getattr(self, "_sess", None):
             self.lib.llx_session_destroy(self._sess)
             self._sess = None
@@ -494,7 +506,7 @@ class LlxSampling(C.Structure):
 class CudaServe:
     """A model served over a paged KV cache (llx_serve_*): sequences of different lengths share each
     step and one pool of pages.  `model` is a loaded CudaModel (fuse=True, one GPU), whose weights it
-    uses and which has to stay open.
+    uses; closing the model closes this too.
 
     `step` takes any number of new tokens per sequence and returns one next token each; `fork` lets
     several answers go on from one prompt, `free` gives a slot back.  Tokens and logits are those of
@@ -505,14 +517,22 @@ class CudaServe:
     def __init__(self, model: CudaModel, *, max_seqs: int, n_pages: int, page_size: int = 64, max_rows: int = 1024) -> None:
         self.model, self.lib = model, model.lib
         self.max_seqs, self.n_pages, self.page_size, self.max_rows = int(max_seqs), int(n_pages), int(page_size), int(max_rows)
-        self._h = C.c_void_p()
+        h = C.c_void_p()
         _check(self.lib, self.lib.llx_serve_create(model._model, self.max_seqs, self.n_pages, self.page_size, self.max_rows,
-                                                   C.byref(self._h)))
+                                                   C.byref(h)))
+        self._serve = h
+        model._users.add(self)
+
+    @property
+    def _h(self) -> C.c_void_p:
+        if not self._serve:
+            raise ValueError("this CudaServe is closed, or its model is")
+        return self._serve
 
     def close(self) -> None:
-        if getattr(self, "_h", None):
-            self.lib.llx_serve_destroy(self._h)
-            self._h = None
+        if getattr(self, "_serve", None):
+            self.lib.llx_serve_destroy(self._serve)
+            self._serve = None
 
     def __del__(self):  # pragma: no cover
         try:
