@@ -1,5 +1,5 @@
 """Builds the CUDA backend in-tree: llaccel_b200/csrc/*.cu -> llaccel_b200/_lib/libllx.so, and where
-torch is installed the binding of the paged calls, csrc/torch_calls.cpp -> _lib/torch_calls.so.
+a torch with CUDA is installed the binding of the paged calls, csrc/torch_calls.cpp -> _lib/torch_calls.so.
 
     python -m llaccel_b200.build [--force]
 
@@ -58,8 +58,16 @@ def lib_up_to_date() -> bool:
     return _newer(LIB, deps())
 
 
+def cuda_torch() -> Path | None:
+    """The folder of the installed torch if that is built with CUDA (looked up without importing it).
+    Any other has no CUDA tensors to bind, nor the libraries to link with."""
+    spec = importlib.util.find_spec("torch")
+    root = Path(spec.origin).parent if spec is not None and spec.origin else None
+    return root if root is not None and (root / "lib" / "libc10_cuda.so").exists() else None
+
+
 def calls_up_to_date() -> bool:
-    if importlib.util.find_spec("torch") is None:
+    if cuda_torch() is None:
         return True
     return _newer(CALLS, [CSRC / "torch_calls.cpp", *INCLUDE.glob("*.h")])
 
@@ -115,11 +123,11 @@ def _compile(verbose: bool) -> Path:
 
 
 def _compile_calls(verbose: bool) -> None:
-    if importlib.util.find_spec("torch") is None:
+    root = cuda_torch()
+    if root is None:
         return
     import torch
 
-    root = Path(torch.__file__).parent
     tmp = CALLS.with_suffix(f".so.{os.getpid()}.tmp")
     cuda = Path(nvcc()).resolve().parent.parent
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
