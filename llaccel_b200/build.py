@@ -66,10 +66,17 @@ def cuda_torch() -> Path | None:
     return root if root is not None and (root / "lib" / "libc10_cuda.so").exists() else None
 
 
+def _made_for(root: Path) -> str:
+    """What the binding depends on besides its sources: the torch in `root` and this Python."""
+    return f"{(root / 'version.py').read_text()}{sysconfig.get_config_var('EXT_SUFFIX')}\n"
+
+
 def calls_up_to_date() -> bool:
-    if cuda_torch() is None:
+    root = cuda_torch()
+    if root is None:
         return True
-    return _newer(CALLS, [CSRC / "torch_calls.cpp", *INCLUDE.glob("*.h")])
+    note = CALLS.with_suffix(".torch")
+    return _newer(CALLS, [CSRC / "torch_calls.cpp", *INCLUDE.glob("*.h")]) and note.exists() and note.read_text() == _made_for(root)
 
 
 def up_to_date() -> bool:
@@ -140,6 +147,7 @@ def _compile_calls(verbose: bool) -> None:
     if r.returncode != 0:
         raise RuntimeError(f"g++ failed on torch_calls.cpp:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, CALLS)
+    CALLS.with_suffix(".torch").write_text(_made_for(root))
 
 
 def main(argv=None) -> None:

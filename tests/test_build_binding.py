@@ -5,6 +5,8 @@ import os
 import subprocess
 import sys
 
+import pytest
+
 from conftest import REPO
 
 
@@ -30,3 +32,12 @@ def up_to_date(folder, binding) -> bool:
 def test_a_torch_without_cuda_needs_no_binding(tmp_path):
     assert up_to_date(stand_in(tmp_path / "cpu", "2.11.0+cpu", cuda=False), tmp_path / "none.so")
     assert not up_to_date(stand_in(tmp_path / "gpu", "2.11.0+cu128", cuda=True), tmp_path / "none.so")
+
+
+def test_another_torch_needs_another_binding(tmp_path):
+    from llaccel_b200 import build
+    build.build()
+    if not build.CALLS.exists():
+        pytest.skip("no binding here")
+    assert build.calls_up_to_date()
+    assert not up_to_date(stand_in(tmp_path, "2.99.0+cu130", cuda=True), build.CALLS)
