@@ -2,6 +2,7 @@
 // the caller's stream.  Nothing is allocated, synchronised or remembered between calls.
 #include "paged.h"
 
+#include <climits>
 #include <string>
 
 namespace llx {
@@ -50,17 +51,20 @@ void need_rows(int64_t rows, int64_t n_heads, int64_t n_kv_heads, int64_t n_seqs
   need(q_start != nullptr && length != nullptr, "null q_start or length");
 }
 
-// the caller's current device, put back when the call ends
+// makes `device` current; the caller's is put back when the call ends
 class OnDevice {
  public:
   explicit OnDevice(int64_t device) {
     int now = -1;
-    if (cudaGetDevice(&now) != cudaSuccess) return;
-    if (now != device && cudaSetDevice((int)device) == cudaSuccess) back_ = now;
+    error = cudaGetDevice(&now);
+    if (error != cudaSuccess || now == device) return;
+    error = cudaSetDevice((int)device);
+    if (error == cudaSuccess) back_ = now;
   }
   ~OnDevice() {
     if (back_ >= 0) cudaSetDevice(back_);
   }
+  cudaError_t error;
 
  private:
   int back_ = -1;
@@ -70,10 +74,10 @@ template <class Args, class Check, class Launch>
 llx_status call(const char* name, const Args* a, void* stream, Check check, Launch launch) {
   try {
     need(a != nullptr, "null argument");
-    need(a->device >= 0, "no such device");
+    need(a->device >= 0 && a->device <= INT_MAX, "no such device");
     check(*a);
     OnDevice on(a->device);
-    const cudaError_t e = launch(*a, static_cast<cudaStream_t>(stream));
+    const cudaError_t e = on.error != cudaSuccess ? on.error : launch(*a, static_cast<cudaStream_t>(stream));
     if (e == cudaSuccess) return LLX_OK;
     cudaGetLastError();  // reported here, not by the caller's next call
     noalloc_set_error(std::string(name) + ": " + cudaGetErrorString(e));

@@ -71,3 +71,30 @@ def test_a_fork_of_a_page_that_is_not_there_changes_nothing(paged, share, bad):
     assert int(status.item()) == 0 and length.tolist() == [20, 16, 20, 20, 16]
     new = table[3, 1].long()
     assert torch.equal(k[:, new, :, :4], before[0][:, 0, :, :4])
+
+
+@pytest.mark.parametrize("name", ["llx_paged_append", "llx_paged_attention", "llx_pages_fork", "llx_sample"])
+def test_a_device_that_is_not_there_is_refused(paged, name):
+    """Not run on the current one instead."""
+    from test_paged_host import call
+    lib = paged.load_library()
+    for device in (1000, 1 << 31, (1 << 32) + 1):
+        assert call(lib, name, device=device) in (1, 3)  # LLX_ERR_INVALID, LLX_ERR_CUDA
+        assert lib.llx_last_error().decode().startswith(name + ": ")
+
+
+@gpu
+def test_a_call_for_a_device_that_is_not_there_changes_nothing(paged):
+    lib = paged.load_library()
+    table, length, refs, slots = ints([[0, 1], [2, -1]]), ints([20, 3]), ints([1, 1, 1]), ints([0, 1])
+
+    def free(device):
+        pack = (0, 0, 0, 256, 1, 3, 1, 16, 16, table.data_ptr(), 2, 2, 2, length.data_ptr(), refs.data_ptr(), slots.data_ptr(), 0, 2,
+                0, 0, 0, 0, 0, device)
+        code = lib.llx_pages_free(paged._PAGES.pack(*pack), torch.cuda.current_stream().cuda_stream)
+        torch.cuda.synchronize()
+        return code
+
+    assert free(torch.cuda.device_count()) == 3 and length.tolist() == [20, 3] and refs.tolist() == [1, 1, 1]
+    assert torch.cuda.current_device() == 0
+    assert free(0) == 0 and length.tolist() == [0, 0] and refs.tolist() == [0, 0, 0]
