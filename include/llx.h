@@ -192,7 +192,7 @@ llx_status llx_linear_argmax_noalloc(const int8_t* A, const int8_t* W, const int
  * CUDA device of the pointers and of the stream; the caller's current device is left as it was.
  * Every field is 8 bytes wide. */
 #define LLX_STATUS_BAD_PAGE 1      /* a position whose page id is outside the cache */
-#define LLX_STATUS_BAD_POSITION 2  /* a position below 0, or beyond the rotation or page tables */
+#define LLX_STATUS_BAD_POSITION 2  /* a position below 0, or beyond the rotation or page tables or 31 bits */
 #define LLX_STATUS_BAD_BOUND 4     /* a sequence with more rows or positions than the call was told */
 #define LLX_STATUS_NO_PAGES 8      /* too few free pages: nothing was changed */
 #define LLX_STATUS_BAD_SLOT 16     /* a slot outside the table, listed twice, or both parent and child */

@@ -401,7 +401,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_reserve(const llx_pages_
     if (i < a.n) {
       const int s = a.list_a[i];
       const int64_t len = a.length[s], more = a.list_b[i];
-      if (len < 0 || more < 0 || len + more > a.max_pages * P) {
+      if (len < 0 || more < 0 || len + more > a.max_pages * P || len + more > INT32_MAX) {
         atomicOr(&code, LLX_STATUS_BAD_POSITION);
       } else {
         mine = pages_for(len + more, P) - pages_for(len, P);

@@ -84,7 +84,7 @@ class Pages:
         P, code, want = self.P, 0, []
         for s, c in zip(slots, counts):
             n = int(self.length[s])
-            if n < 0 or c < 0 or n + c > self.table.shape[1] * P:
+            if n < 0 or c < 0 or n + c > min(self.table.shape[1] * P, 2 ** 31 - 1):
                 code |= 2
                 continue
             if c and n % P:

@@ -98,3 +98,16 @@ def test_a_call_for_a_device_that_is_not_there_changes_nothing(paged):
     assert free(torch.cuda.device_count()) == 3 and length.tolist() == [20, 3] and refs.tolist() == [1, 1, 1]
     assert torch.cuda.current_device() == 0
     assert free(0) == 0 and length.tolist() == [0, 0] and refs.tolist() == [0, 0, 0]
+
+
+@gpu
+def test_lengths_end_at_31_bits(paged):
+    """A table row of 2^24 pages of 256 holds more positions than an int32 length can count."""
+    W, P, status = 1 << 24, 256, ints([0])
+    table = torch.full((1, W), -1, dtype=torch.int32, device="cuda")
+    table[0, (2 ** 31 - 10) // P] = 0
+    length, refs = ints([2 ** 31 - 10]), ints([1, 0])
+    paged.reserve(table, length, refs, ints([0]), ints([10]), P, status=status)
+    assert int(status.item()) == 2 and length.tolist() == [2 ** 31 - 10] and refs.tolist() == [1, 0]
+    paged.reserve(table, length, refs, ints([0]), ints([9]), P, status=status.zero_())
+    assert int(status.item()) == 0 and length.tolist() == [2 ** 31 - 1] and refs.tolist() == [1, 0]
