@@ -40,7 +40,7 @@ __global__ void __launch_bounds__(256) k_paged_attention_any(const llx_paged_att
   const int64_t P = a.page_size;
   int code = sv.code;
   // keys 0 .. T - 1; the bounds of the call and of the page table cut both
-  int64_t T = sv.slot < 0 ? 0 : sv.len - sv.rows + (r - sv.first) + 1;
+  int64_t T = sv.slot < 0 ? 0 : (int64_t)sv.len - sv.rows + (r - sv.first) + 1;
   if (T <= 0 && !code) code = LLX_STATUS_BAD_POSITION;
   if (r - sv.first >= a.max_rows) {
     if (threadIdx.x == 0) raise_status(a.status, LLX_STATUS_BAD_BOUND);

@@ -111,3 +111,12 @@ def test_lengths_end_at_31_bits(paged):
     assert int(status.item()) == 2 and length.tolist() == [2 ** 31 - 10] and refs.tolist() == [1, 0]
     paged.reserve(table, length, refs, ints([0]), ints([9]), P, status=status.zero_())
     assert int(status.item()) == 0 and length.tolist() == [2 ** 31 - 1] and refs.tolist() == [1, 0]
+
+
+@gpu
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("rows", [[1, 1], [3, 40]])
+def test_the_lowest_length_has_no_keys(paged, rows, D):
+    """-2^31 less the launch's rows does not become a long context."""
+    from test_paged_ops import attention_case
+    assert attention_case(np.random.default_rng(D), 4, 2, D, 16, rows, [-2 ** 31, 40]) == 2
