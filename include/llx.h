@@ -230,8 +230,8 @@ llx_status llx_paged_append(const llx_paged_append_args* a, void* stream);
 /* Causal attention of the launch's rows over their sequences' pages: q8 -> out, both
  * [rows][n_heads][head_dim] i8 (16-byte aligned rows).  score: z = mulshift(max - s, Ms, Ss),
  * output: mulshift(o, Mo, So), prob_bits 8 or 15.  Keys whose page id is outside the cache count
- * as absent; a row without keys gets zeros.  max_rows and max_len bound every sequence's rows and
- * length (they size the launch; rows and positions beyond them are not computed). */
+ * as absent; a row without keys gets zeros.  max_rows and max_len bound the rows and the length of every
+ * sequence that has rows (they size the launch; rows and positions beyond them are not computed). */
 typedef struct {
   const int8_t* q8;
   int8_t* out;

@@ -134,8 +134,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int cap = key_cap(a);
   if (blockIdx.x == 0 && kvh == 0 && tid == 0) {
     int code = sv.code;
-    if (sv.rows > a.max_rows || sv.len > cap) code |= LLX_STATUS_BAD_BOUND;
-    if (!code && sv.len < sv.rows) code = LLX_STATUS_BAD_POSITION;
+    if (sv.rows > a.max_rows || (sv.rows && sv.len > cap)) code |= LLX_STATUS_BAD_BOUND;
+    if (!code && sv.rows && sv.len < sv.rows) code = LLX_STATUS_BAD_POSITION;
     if (code) raise_status(a.status, code);
   }
   if (tile < 0) return;

@@ -120,3 +120,13 @@ def test_the_lowest_length_has_no_keys(paged, rows, D):
     """-2^31 less the launch's rows does not become a long context."""
     from test_paged_ops import attention_case
     assert attention_case(np.random.default_rng(D), 4, 2, D, 16, rows, [-2 ** 31, 40]) == 2
+
+
+@gpu
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("rows", [[0, 1, 0], [0, 40, 0]])
+def test_bounds_are_those_of_sequences_with_rows(paged, rows, D):
+    """A slot that brings none may be longer than max_len (or hold a length of no sense): nothing of it is computed."""
+    from test_paged_ops import attention_case
+    assert attention_case(np.random.default_rng(D), 4, 2, D, 16, rows, [100, 50, -7], max_len=50) == 0
+    assert attention_case(np.random.default_rng(D), 4, 2, D, 16, rows, [100, 50, -7], max_len=49) == 4
