@@ -121,7 +121,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   for (int x = tid; x < 1024; x += kThreads)
     reinterpret_cast<uint4*>(base + L::curve)[x] = reinterpret_cast<const uint4*>(kDevCurve)[x];
   __syncthreads();  // any_bad is clear before a thread sets it
-  pdl_trigger();
   pdl_wait();
   const int i = blockIdx.z, kvh = blockIdx.y;
   const SeqView sv = view_sequence(a, i);
@@ -168,6 +167,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc::tc_fence_after();
   const uint32_t tmem = tmem_s;
+  // Dependents launch once every CTA has its TMEM columns or has left: a GEMM that follows takes columns
+  // before it waits for this grid, and a CTA here that found too few left would wait for it in turn.
+  pdl_trigger();
   if (tid == 0 && any_bad) raise_status(a.status, LLX_STATUS_BAD_PAGE);
 
   if (warp < 2) {
