@@ -298,25 +298,25 @@ cudaError_t launch_paged_append(const llx_paged_append_args& a, cudaStream_t st)
 constexpr int kPlanThreads = 1024;
 constexpr int kMaxSlots = 1 << 18;  // slots of a table (bitmap of 32 KB)
 
-// exclusive sum over the block; *total gets the whole.  In 64 bits: a slot may ask for 2^24 pages, so the
-// threads of one round for 2^34, and a request must not wrap into one that can be met.
-__device__ int64_t block_scan(int64_t v, int64_t* total) {
-  __shared__ int64_t part[kPlanThreads / 32];
+// exclusive sum over the block; *total gets the whole
+template <class T>
+__device__ __forceinline__ T block_scan_of(T v, T* total) {
+  __shared__ T part[kPlanThreads / 32];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  int64_t x = v;
+  T x = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+    const T y = __shfl_up_sync(0xffffffffu, x, o);
     if (lane >= o) x += y;
   }
   __syncthreads();  // part may still be read by an earlier call
   if (lane == 31) part[w] = x;
   __syncthreads();
   if (w == 0) {
-    int64_t y = part[lane];
+    T y = part[lane];
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t z = __shfl_up_sync(0xffffffffu, y, o);
+      const T z = __shfl_up_sync(0xffffffffu, y, o);
       if (lane >= o) y += z;
     }
     part[lane] = y;
@@ -325,6 +325,11 @@ __device__ int64_t block_scan(int64_t v, int64_t* total) {
   *total = part[kPlanThreads / 32 - 1];
   return x - v + (w ? part[w - 1] : 0);
 }
+// of what slots ask for: 2^24 pages each, so the threads of one round for 2^34, and a request must not wrap
+// into one that can be met
+__device__ int64_t block_scan(int64_t v, int64_t* total) { return block_scan_of(v, total); }
+// of what is known to be at most the cache's pages
+__device__ int page_scan(int v, int* total) { return block_scan_of(v, total); }
 
 __device__ __forceinline__ int64_t pages_for(int64_t len, int64_t P) { return (len + P - 1) / P; }
 
@@ -373,9 +378,9 @@ __device__ void count_pages(const llx_pages_args& a, const int32_t* slots, int s
 __device__ bool take_free(const llx_pages_args& a, int64_t need) {
   const int64_t per = (a.n_pages + kPlanThreads - 1) / kPlanThreads;
   const int64_t p0 = threadIdx.x * per, p1 = p0 + per < a.n_pages ? p0 + per : a.n_pages;
-  int64_t mine = 0, have;
+  int mine = 0, have;
   for (int64_t p = p0; p < p1; ++p) mine += a.refs[p] <= 0;
-  int64_t at = block_scan(mine, &have);
+  int at = page_scan(mine, &have);
   if (have < need) return false;
   for (int64_t p = p0; p < p1 && at < need; ++p)
     if (a.refs[p] <= 0) a.scratch[at++] = (int32_t)p;
@@ -423,15 +428,15 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_reserve(const llx_pages_
   int64_t base = 0;
   for (int64_t i0 = 0; i0 < a.n; i0 += kPlanThreads) {
     const int64_t i = i0 + threadIdx.x;
-    int s = 0;
-    int64_t len = 0, mine = 0, sum;
+    int s = 0, mine = 0, sum;
+    int64_t len = 0;
     if (i < a.n) {
       s = a.list_a[i];
       len = a.length[s];
-      mine = pages_for(len + a.list_b[i], P) - pages_for(len, P);
+      mine = (int)(pages_for(len + a.list_b[i], P) - pages_for(len, P));
     }
-    const int64_t at = base + block_scan(mine, &sum);
-    for (int64_t j = 0; j < mine; ++j) {
+    const int64_t at = base + page_scan(mine, &sum);
+    for (int j = 0; j < mine; ++j) {
       const int id = a.scratch[at + j];
       a.table[s * a.table_stride + pages_for(len, P) + j] = id;
       a.refs[id] = 1;
@@ -466,6 +471,8 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_fork(const llx_pages_arg
   pdl_wait();
   // scratch: the copies' targets [0, N), sources [N, 2N) and rows [2N, 3N), and [3N] their number
   int32_t* done = a.scratch + 3 * a.n_pages;
+  __shared__ int bad;  // a page to be copied is not there
+  if (threadIdx.x == 0) bad = 0;
   if (!lists_fine(a, a.list_b, a.list_a)) {
     if (threadIdx.x == 0) {
       raise_status(a.status, LLX_STATUS_BAD_SLOT);
@@ -476,9 +483,6 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_fork(const llx_pages_arg
   const int64_t P = a.page_size;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // what is to be copied has to be there, before anything is changed
-  __shared__ int bad;
-  if (threadIdx.x == 0) bad = 0;
-  __syncthreads();
   auto there = [&](int slot, int64_t j) {
     const int id = a.table[slot * a.table_stride + j];
     if (id < 0 || id >= a.n_pages) bad = 1;
@@ -495,13 +499,14 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_fork(const llx_pages_arg
     block_scan(mine, &sum);
     need += sum;
   }
-  if (!a.share)
+  if (!a.share) {
     for (int64_t i = warp; i < a.n; i += kPlanThreads / 32) {
       const int64_t held = pages_for(slot_length(a, a.list_a[i]), P);
       for (int64_t j = lane; j < held; j += 32) there(a.list_a[i], j);
     }
-  __syncthreads();
-  if (bad) {
+    __syncthreads();
+  }
+  if (bad) {  // block_scan's barriers lie between
     if (threadIdx.x == 0) {
       raise_status(a.status, LLX_STATUS_BAD_PAGE);
       *done = 0;
@@ -521,12 +526,12 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_fork(const llx_pages_arg
   int64_t base = 0;
   for (int64_t i0 = 0; i0 < a.n; i0 += kPlanThreads) {
     const int64_t i = i0 + threadIdx.x;
-    int64_t mine = 0, sum;
+    int mine = 0, sum;
     if (i < a.n) {
       const int64_t len = slot_length(a, a.list_a[i]);
-      mine = pages_for(len, P) - (a.share ? len / P : 0);
+      mine = (int)(pages_for(len, P) - (a.share ? len / P : 0));
     }
-    first[threadIdx.x] = (int)block_scan(mine, &sum);  // below `need`, which is at most n_pages
+    first[threadIdx.x] = page_scan(mine, &sum);
     __syncthreads();
     for (int64_t x = warp; x < kPlanThreads && i0 + x < a.n; x += kPlanThreads / 32) {
       const int from = a.list_a[i0 + x], to = a.list_b[i0 + x];
@@ -612,10 +617,9 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_compact(const llx_pages_
   const int64_t N = a.n_pages, per = (N + kPlanThreads - 1) / kPlanThreads;
   const int64_t p0 = min(N, threadIdx.x * per), p1 = min(N, p0 + per);
   int32_t *to = a.scratch, *src = to + N, *dst = src + N;
-  int64_t used = 0, all;
+  int used = 0, live;
   for (int64_t p = p0; p < p1; ++p) used += a.refs[p] > 0;
-  const int before = (int)block_scan(used, &all);  // live pages below p0
-  const int live = (int)all;
+  const int before = page_scan(used, &live);  // live pages below p0
   // movers: live pages from id `live` on; holes: free pages below it; as many of each.  Of the pages
   // below `live`, those that are not live are holes; of the live pages, those past the ones below it move.
   __shared__ int live_below;  // live pages with an id below `live`
