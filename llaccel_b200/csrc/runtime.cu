@@ -1571,6 +1571,7 @@ static void ensure_i16(llx_session* s, size_t n) {
   LLX_CUDA(cudaStreamSynchronize(s->st));
   if (s->h_i16) cudaFreeHost(s->h_i16);
   s->h_i16 = nullptr;
+  s->h_i16_n = 0;
   LLX_CUDA(cudaMallocHost(&s->h_i16, n * sizeof(int16_t)));
   s->h_i16_n = n;
 }

@@ -206,6 +206,16 @@ static void compactions(llx_model* m, cudaError_t e) {
   }
 }
 
+// a buffer that could not be made larger is not taken for the one it was
+static void logits_buffer(llx_model* m) {
+  for (int n = 1; n < 5; ++n) {
+    Serve s(m);
+    CHECK(s.step({0}) == LLX_OK);
+    if (failing(n, cudaErrorMemoryAllocation, [&] { return s.step({0, 1}); }) == LLX_OK) break;
+    CHECK(!reserved && s.step({0}) == LLX_OK && s.step({0, 1}) == LLX_OK);
+  }
+}
+
 int main(int argc, char** argv) {
   llx_model* m = nullptr;
   if (argc < 2 || llx_model_load(argv[1], nullptr, &m) != LLX_OK) return printf("load: %s\n", llx_last_error()), 1;
@@ -216,6 +226,7 @@ int main(int argc, char** argv) {
     compactions(m, e);
   }
   too_few_pages(m);
+  logits_buffer(m);
   llx_model_destroy(m);
   printf("%d failures\n", failures);
   return failures != 0;
