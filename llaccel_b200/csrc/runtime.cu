@@ -1999,6 +1999,7 @@ static llx_status guarded(F&& f) {
     f();
     return LLX_OK;
   } catch (const Error& e) {
+    cudaGetLastError();  // reported here, not by the next call's launches
     g_err = e.what();
     return e.code;
   } catch (const std::bad_alloc&) {
