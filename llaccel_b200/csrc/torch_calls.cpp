@@ -154,7 +154,7 @@ PyObject* append(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const at::Tensor &q = in.tensor(kI16), &k = in.tensor(kI16), &v = in.tensor(kI8), &kp = in.tensor(kI8), &vp = in.tensor(kI8);
     const at::Tensor &table = in.tensor(kI32), &length = in.tensor(kI32), &q_start = in.tensor(kI32);
     const at::Tensor &cos = in.tensor(kI16), &sin = in.tensor(kI16);
-    need(q.dim() == 3);
+    need(q.dim() == 3 && q.size(0) > 0);  // tensors without rows have no addresses
     const int64_t R = q.size(0), H = q.size(1), D = q.size(2);
     in.pair(a.q_M, a.q_S);
     in.pair(a.k_M, a.k_S);
@@ -195,7 +195,7 @@ PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const at::Tensor* seqs = in.maybe(kI32);
     const at::Tensor& out = in.tensor(kI8);
     const at::Tensor* status = in.maybe(kI32);
-    need(q8.dim() == 3);
+    need(q8.dim() == 3 && q8.size(0) > 0);
     const int64_t R = q8.size(0), H = q8.size(1), D = q8.size(2);
     put_pages(a, kp, vp, D);
     put_launch(a, table, length, q_start, seqs, status);

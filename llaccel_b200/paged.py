@@ -188,7 +188,8 @@ def _append_checked(q, k, v, k_pages, v_pages, table, length, q_start, cos, sin,
                         qe, qC, qsh, ke, kC, ksh, cos.data_ptr(), sin.data_ptr(), rot[0], *q_rq, *k_rq,
                         k_pages.data_ptr(), v_pages.data_ptr(), page_stride, n_pages, P, *_table(table, length),
                         length.data_ptr(), starts, slots, n, status.data_ptr() if status is not None else 0, dev)
-    return (_lib or _load()).llx_paged_append(args, _stream(dev))
+    # a launch without rows is nothing to do, and its tensors have no addresses to check
+    return (_lib or _load()).llx_paged_append(args, _stream(dev)) if R else 0
 
 
 def attention(q8, k_pages, v_pages, table, length, q_start, score_rq, out_rq, *, prob_bits=15, max_rows, max_len,
@@ -230,7 +231,8 @@ def _attention_checked(q8, k_pages, v_pages, table, length, q_start, score_rq, o
                            k_pages.data_ptr(), v_pages.data_ptr(), page_stride, n_pages, P, *_table(table, length),
                            length.data_ptr(), starts, slots, n, max_rows, max_len, *score_rq, *out_rq, prob_bits,
                            status.data_ptr() if status is not None else 0, dev)
-    return (_lib or _load()).llx_paged_attention(args, _stream(dev))
+    # a launch without rows is nothing to do, and its tensors have no addresses to check
+    return (_lib or _load()).llx_paged_attention(args, _stream(dev)) if R else 0
 
 
 def _page_call(name, pool, table, length, refs, list_a, list_b, share, new_table, new_refs, status) -> None:

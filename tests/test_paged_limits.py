@@ -130,3 +130,30 @@ def test_bounds_are_those_of_sequences_with_rows(paged, rows, D):
     from test_paged_ops import attention_case
     assert attention_case(np.random.default_rng(D), 4, 2, D, 16, rows, [100, 50, -7], max_len=50) == 0
     assert attention_case(np.random.default_rng(D), 4, 2, D, 16, rows, [100, 50, -7], max_len=49) == 4
+
+
+@gpu
+@pytest.mark.parametrize("D", [32, 64])
+def test_launches_without_rows(paged, D):
+    """No rows (of no sequence, or of two that bring none), no slots, nothing to sample: nothing to do."""
+    from llaccel_b200 import sampling
+    H, Hkv, P = 4, 2, 16
+    pages = [torch.full((3, Hkv, P, D), 5, dtype=torch.int8, device="cuda") for _ in "kv"]
+    table, length, status = ints([[0], [1]]), ints([3, 0]), ints([0])
+    cos, sin = (torch.zeros((20, D // 2), dtype=torch.int16, device="cuda") for _ in "cs")
+    for q_start, seqs in (([0], None), ([0, 0, 0], None), ([0, 0, 0], ints([1, 0])), ([0], ints([]))):
+        new = [torch.zeros((0, h, D), dtype=t, device="cuda") for h, t in ((H, torch.int16), (Hkv, torch.int16), (Hkv, torch.int8))]
+        q8 = paged.append(*new, *pages, table, length, ints(q_start), cos, sin, (1 << 30, 33), (1 << 30, 33), seqs=seqs, status=status)
+        o = paged.attention(q8, *pages, table, length, ints(q_start), (1 << 30, 33), (1 << 30, 33), max_rows=0, max_len=3, seqs=seqs,
+                            status=status)
+        assert q8.shape == o.shape == (0, H, D) and o.dtype == torch.int8
+    with pytest.raises(ValueError, match="must be"):
+        paged.attention(q8, *pages, table, length, ints([0]).long(), (1, 33), (1, 33), max_rows=0, max_len=3)
+    refs = ints([1, 0, 0])
+    paged.reserve(table, length, refs, ints([]), ints([]), P, status=status)
+    paged.fork(*pages, table, length, refs, ints([]), ints([]), status=status)
+    paged.free(table, length, refs, ints([]), status=status)
+    token, prob = sampling.sample(torch.zeros((0, 9), dtype=torch.int16, device="cuda"), torch.zeros(0, dtype=torch.float64, device="cuda"),
+                                  exponent=-3)
+    assert len(token) == len(prob) == 0
+    assert int(status.item()) == 0 and length.tolist() == [3, 0] and refs.tolist() == [1, 0, 0] and all(int(p.min()) == 5 for p in pages)
