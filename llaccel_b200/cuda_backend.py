@@ -607,14 +607,19 @@ class CudaServe:
 
     def generate(self, prompts, n_tokens: int, *, rng=None, chunk: int | None = None, **settings) -> list[list[int]]:
         """`n_tokens` new tokens after each of the prompts (any lengths, at most max_seqs of them), greedy
-        or, with `rng` (a numpy Generator), sampled with `settings`.  Prompts go in by chunks of at
-        most `chunk` tokens (default: what a step's rows allow), while others already decode.  Uses
-        slots 0 .. len(prompts) - 1 and gives them back."""
+        or, with `rng` (a numpy Generator), sampled with `settings` (per prompt, or one for all).
+        Prompts go in by chunks of at most `chunk` tokens (default, and 0: what a step's rows allow),
+        while others already decode.  Uses slots 0 .. len(prompts) - 1 and gives them back."""
         P = [self.model._validate(p, n_tokens) for p in prompts]
         if len(P) > self.max_seqs:
             raise ValueError(f"{len(P)} prompts, but {self.max_seqs} slots")
         if len(P) > self.max_rows:
             raise ValueError(f"{len(P)} prompts, but steps of {self.max_rows} rows")
+        if chunk is not None and chunk < 0:
+            raise ValueError("a chunk cannot be negative")
+        if rng is None and any(value is not None for value in settings.values()):
+            raise ValueError("sampling needs random numbers")
+        each = {name: np.broadcast_to(np.asarray(value), (len(P),)) for name, value in settings.items() if value is not None}
         out: list[list[int]] = [[] for _ in P]
         left = [list(p) for p in P]
         self.free(range(len(P)))
@@ -628,7 +633,7 @@ class CudaServe:
                     slots.append(i)
                     feed.append(left[i][:take])
                     left[i] = left[i][take:]
-                extra = dict(random=rng.random(len(slots)), **settings) if rng is not None else {}
+                extra = dict(random=rng.random(len(slots)), **{k: a[live] for k, a in each.items()}) if rng is not None else {}
                 got = self.step(slots, feed, **extra)["next"]
                 for i, t in zip(slots, got):
                     if not left[i]:
