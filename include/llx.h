@@ -231,7 +231,8 @@ llx_status llx_paged_append(const llx_paged_append_args* a, void* stream);
  * [rows][n_heads][head_dim] i8 (16-byte aligned rows).  score: z = mulshift(max - s, Ms, Ss),
  * output: mulshift(o, Mo, So), prob_bits 8 or 15.  Keys whose page id is outside the cache count
  * as absent; a row without keys gets zeros.  max_rows and max_len bound the rows and the length of every
- * sequence that has rows (they size the launch; rows and positions beyond them are not computed). */
+ * sequence that has rows (they size the launch and choose the kernel; rows and positions beyond them
+ * are not computed). */
 typedef struct {
   const int8_t* q8;
   int8_t* out;
@@ -257,8 +258,10 @@ llx_status llx_paged_attention(const llx_paged_attention_args* a, void* stream);
  *            becomes its parent's copy: with share, full pages are shared and a part-filled last
  *            page is copied; without, every page is copied.  Rows past the parent's length are
  *            not copied.  A child may be listed once and may not be a parent.  All or nothing.
- *   free:    list_a = slots; their pages are released, their lengths set to 0.
- *   compact: live pages move to the lowest ids, in order; new_table / new_refs receive the
+ *   free:    list_a = slots; their pages are released, their lengths set to 0.  Slots outside the table
+ *            are skipped and noted; the others are freed all the same.
+ *   compact: live pages come to the lowest ids: of n live pages those with an id from n on move, in
+ *            order, into the free ids below n, the others stay; new_table / new_refs receive the
  *            renamed table (same strides as table) and counts, and may be table and refs.
  * scratch: llx_pages_scratch(n_pages) bytes of device memory, used until the call's work is done. */
 typedef struct {

@@ -105,10 +105,13 @@ __global__ void __launch_bounds__(256) k_paged_append_any(const llx_paged_append
 // head, each with 8 neighbouring values and their 8 partners half a head away: one 16-byte load each,
 // and a rotation without exchange.  The row's place is looked up while those loads are under way.
 // Per row 2 (H + Hkv) D + Hkv D bytes read, H D + 2 Hkv D written.  8,000 rows of 16 + 8 heads of 128 with
-// norms: 92 MB in 37 us, 2.5 TB/s; its instructions bound it (65 % of the issue slots; 64-bit products of
-// norm and requantization, some 40 instructions a value), the copy rate would allow 14 us.  A block per
-// row and a warp per head with single loads took 166; one lane per head for square root and quotient, after
-// a first reading of the row, 47.  A single row takes 3.2 us inside a graph, most of it latency.
+// norms: 92 MB in 37 us, 2.5 TB/s; the copy rate would allow 14 us.  No limit is reached: 65 % of the issue
+// slots, 17 % of DRAM.  64-bit products of norm and requantization make some 40 instructions a value; 80
+// registers leave five warps a scheduler, which wait 1.6 cycles an instruction for results, 1.3 for the
+// integer multipliers and 0.8 for loads, over 2.3 waves.  A block per row and a warp per head with single
+// loads took 166; one lane per head for square root and quotient, after a first reading of the row, 47.  A
+// single row takes 3.2 us inside a graph, most of it latency.  Other head sizes and alignments:
+// k_paged_append_any, 8,000 rows of 16 + 8 heads of 96 in 178 us (68 MB).
 struct AppendSide {
   const int16_t *x, *gamma;
   int64_t eps, C, stride;
@@ -388,6 +391,8 @@ __device__ bool take_free(const llx_pages_args& a, int64_t need) {
   return true;
 }
 
+// 64 slots, one position each, of 8,192 pages: 6.1 us in a graph, 10.8 a call from Python; the same block's
+// chain as a fork's.
 __global__ void __launch_bounds__(kPlanThreads) k_pages_reserve(const llx_pages_args a) {
   pdl_trigger();
   pdl_wait();
@@ -446,6 +451,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_reserve(const llx_pages_
   }
 }
 
+// Not all or nothing: the good slots of a list are freed, the others noted.  2.2 us in a graph for 64 slots.
 __global__ void __launch_bounds__(kPlanThreads) k_pages_free(const llx_pages_args a) {
   pdl_trigger();
   pdl_wait();
@@ -465,7 +471,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_free(const llx_pages_arg
 
 // Children become copies of their parents; the copying itself is k_pages_copy's.  One block decides, so
 // the call is all or nothing without a wait between blocks: 48 children of sequences of 500 to 1,100
-// positions take 15 us with the copying (20 MB, 3 us), most of it this block's chain of scans.
+// positions take 16.1 us with the copying (20 MB, 3 us), most of it this block's chain of scans.
 __global__ void __launch_bounds__(kPlanThreads) k_pages_fork(const llx_pages_args a) {
   pdl_trigger();
   pdl_wait();
@@ -560,7 +566,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_pages_fork(const llx_pages_arg
 
 // Copies pages: block (x, y) takes moves x, x + gridDim.x, ... of layer y / 2, k or v.  `rows` null:
 // whole pages.  Four 16-byte loads per thread are under way before the first is stored; a page of 16 KB
-// per layer is one round.  Bytes bound it: 359 MB copied in 58 us, 0.94 of the copy rate; in place, where
+// per layer is one round.  Bytes bound it: 359 MB copied in 59 us, 0.94 of the copy rate; in place, where
 // pages move within one range (compact, 405 MB), 75 us, 0.82.
 __global__ void __launch_bounds__(256) k_pages_copy(const llx_pages_args a, const int32_t* src, const int32_t* dst,
                                                     const int32_t* rows, const int32_t* number,
@@ -609,6 +615,7 @@ __global__ void __launch_bounds__(256) k_pages_copy(const llx_pages_args a, cons
   }
 }
 
+// The pages from id `live` on move, in order, into the free pages below; the others stay where they are.
 // scratch: [0, N) new id of each page, [N, 2N) holes then sources of the moves, [2N, 3N) their
 // targets, [3N] number of moves
 __global__ void __launch_bounds__(kPlanThreads) k_pages_compact(const llx_pages_args a) {

@@ -23,7 +23,8 @@ __device__ __forceinline__ T reduce_block(T v, T* scratch, Op op) {
 
 // Any geometry (head sizes other than 64 and 128, more sequences than a grid axis holds): one block per
 // (row, query head), three passes over the keys, scores recomputed.  It reads a row's keys three times for
-// every query head and has no reuse between rows: 57.7 ms where the chunk kernel takes 0.27.
+// every query head and has no reuse between rows: 57.7 ms where the chunk kernel takes 0.27; 64 single tokens
+// of 1,000 keys, 14 heads on 2 of 80, 184 us for 20 MB.
 __global__ void __launch_bounds__(256) k_paged_attention_any(const llx_paged_attention_args a) {
   pdl_trigger();
   pdl_wait();
@@ -152,8 +153,13 @@ cudaError_t launch_paged_attention(const llx_paged_attention_args& args, cudaStr
   if (a.max_rows > a.rows) a.max_rows = a.rows;  // grids follow it
   if (a.rows == 0 || a.n_seqs == 0 || a.max_rows == 0) return cudaSuccess;
   const int64_t pairs = a.max_rows * (a.n_heads / a.n_kv_heads);
-  // Up to 32 stacked pairs the cache is read once per 8 of them by the few-row kernel; from there on,
-  // and in launches that mix prompt chunks with single tokens, the chunk kernel takes every sequence.
+  // Up to 32 stacked pairs the cache is read once per 8 of them by the few-row kernel; from there on, and in
+  // launches that mix prompt chunks with single tokens, the chunk kernel takes every sequence.  For mixed
+  // launches two were measured: 30 single tokens of at most 2,300 keys beside 2 chunks, 2 KV heads of 64, 74 us
+  // against 102 for a kernel each; 30 of 4,500 keys beside a chunk of 500, 8 KV heads of 128, 275 against 156
+  // (84 and 72 alone).  So the rule loses where single tokens have long contexts.
+  // It also steps at both of its bounds: 4 sequences of 4 draft rows (28 pairs) over 1,100 keys take 12 us,
+  // of 5 rows (35 pairs) 26; and see paged_decode_fits for max_len.
   constexpr int kFew = 32;
   if (paged_chunk_fits(a)) return pairs <= kFew && paged_decode_fits(a, pairs) ? launch_paged_decode(a, st) : launch_paged_chunk(a, st);
   return launch_k(k_paged_attention_any, dim3((unsigned)a.rows, (unsigned)a.n_heads), dim3(256), 0, st, a);

@@ -21,7 +21,10 @@
 // one block per row and head 57,717 us; this form 494; exponentials from one table 405; whole tiles without
 // masks and cheaper waits 372; the table in words 323; page ids read ahead 303; a second loading warp 273.
 // A tile's keys stay with one CTA: launches of few tiles over long contexts leave SMs idle (14 CTAs for 110
-// rows, 16 heads on 2, about 50k keys: 1.1 ms).
+// rows, 16 heads on 2, about 50k keys: 1.1 ms).  And the grid is the longest chunk's tiles for every sequence
+// and KV head: of some 1,344 CTAs of a mixed launch (2 chunks of 300 to 420 rows, 30 single rows, 74 us) 144 have a
+// tile, and the others, an SM each, set up their barriers and the table before they see that; the chain of
+// the longest tile, 21 tiles of keys, is some 55 us of it.
 // Roles: warps 0 and 1 load (every other stage), warps 2 and 3 issue the MMAs (every other score tile of
 // passes 1 and 2; the scores and the values of pass 3), warps 4 to 19 do the softmax.
 #include <atomic>

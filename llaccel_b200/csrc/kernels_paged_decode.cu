@@ -1,9 +1,9 @@
 // Paged attention of few query rows per sequence (decode steps, a handful of draft tokens).
 //
 // A cluster of C CTAs serves one (sequence, KV head, group of up to 8 stacked (row, head) pairs);
-// each CTA takes a slice of the keys.  Two warps stream the slice's K rows, then its V rows, page by
-// page through a ring of TMA-filled stages (one warp: 84 us and 112 for the
-// launches below); eight warps consume them, so every byte of the cache is read once:
+// each CTA takes a slice of the keys.  Two warps stream the slice's K rows, then its V rows, page by page
+// through a ring of TMA-filled stages (one warp: 84 us and 112 for the launches below); eight warps consume
+// them, so every byte of the cache is read once:
 //   scores  S^T (16 keys x 8 pairs) = K (16 x 32) Q^T per int8 MMA, kept in shared memory;
 //   maxima  of the slices meet in every CTA of the cluster (the reference's global maximum);
 //   table exponentials in place, and their sums meet the same way;
@@ -449,6 +449,11 @@ int64_t longest(const llx_paged_attention_args& a) {
 
 }  // namespace
 
+// A slice's scores stay on chip, so max_len has a limit: with pages of 64 about 88,000 keys at head size 128 and
+// 8 pairs a KV head or more, 101,000 at 7, 181,000 at 4; at head size 64 98,000 at 8.  Beyond it the chunk
+// kernel takes the launch, a CTA per KV head and sequence: 2 single tokens of 80,000 keys, 64 heads on 8 of
+// 128, 214 us here; of 100,000 keys 1,543 there.  It reads the bound only for this choice: 16 single tokens of
+// 2,000 keys under a bound of 131,072 take 43 us there.
 bool paged_decode_fits(const llx_paged_attention_args& a, int64_t pairs) {
   if (a.head_dim != 64 && a.head_dim != 128) return false;
   if (longest(a) > (1 << 19)) return false;  // a slice's keys and sums stay in range
@@ -471,10 +476,13 @@ static cudaError_t launch_decode_t(const llx_paged_attention_args& a, cudaStream
   const int64_t units = a.n_seqs * a.n_kv_heads * groups;
   // How many CTAs share a sequence's keys, and how deep their rings are: the cheapest by this count
   // (bytes and ns).  A wave takes what HBM needs for its bytes (6.5 KB a ns), or what its CTAs do: a
-  // ring's bytes per 1.9 us of loaded latency, 49 B a ns of an SM with one CTA on it, 60 with more.  A
-  // wave's phases cost 6 us where a CTA is alone on its SM, less where others stream meanwhile.  Measured: 64 sequences of 1500 to 4200 keys,
-  // 8 KV heads: one CTA each, ring of 4 82 us, of 2 106; two CTAs, ring of 4 95, of 2 112.  Two of 64k
-  // keys: 10 CTAs, ring of 6 103 us; 9, 6 113; 16, 2 118; 8, 4 127.
+  // ring's bytes per 1.9 us of loaded latency, 49 B a ns of an SM with one CTA on it, 60 with more.  A wave's
+  // phases cost 6 us where a CTA is alone on its SM, less where others stream meanwhile.  The constants come
+  // from two launches.  64 sequences of 1500 to 4200 keys, 8 KV heads: one CTA each, ring of 4 82 us, of 2
+  // 106; two CTAs, ring of 4 95, of 2 112.  Two of 64k keys: 10 CTAs, ring of 6 103 us; 9, 6 113; 16, 2 118;
+  // 8, 4 127.
+  // Lengths are max_len here, the sequences' own being on the device: a bound far above them costs.  16 single
+  // tokens of 2,000 keys, 64 heads on 8 of 128: 21 us with a bound of 2,048, 190 with 80,000.
   double best = 1e30;
   bool waves = false;
   for (int c = 1; c <= kMaxCluster; ++c) {

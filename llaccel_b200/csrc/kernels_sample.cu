@@ -98,9 +98,12 @@ __device__ __forceinline__ SampleRow sample_row(const llx_sample_args& a, int64_
 // of them for the row's bulk far below the cut, so only tokens that can matter are counted: for top-k those
 // up to the gap above, for top-p those heavier than (W - need) / V, because the tokens up to that weight
 // add up to W - need at most and the prefix that reaches `need` has only heavier ones.
-// What bounds it: reading and a row's chain of exchanges (some 2,000 cycles each) for small k, 22 us for
-// a single row; instructions where top-p looks at a whole row, 111 a token and 113 us for 128 such rows,
-// 44 without any filter.  A window of exact levels around a cut estimated from a sample of the tokens saves
+// What bounds it: reading and a row's chain of exchanges (some 1,500 to 2,500 cycles each) for small k;
+// instructions where top-p looks at a whole row, 111 a token and 113 us for 128 such rows, 44 without any
+// filter.  A single row of 151,936 tokens with top-p over 16 CTAs takes 23 us, 41,600 cycles of a CTA in one
+// chain: its slice loaded 2,600, the largest logit exchanged 2,900, weights summed 2,700 and exchanged 2,400,
+// the reach found 1,700, the histogram with its barrier 7,100, bins added over the cluster 5,500, the bin's
+// levels 7,500, kept weights 3,900 and exchanged 1,500, the draw 3,700.  A window of exact levels around a cut estimated from a sample of the tokens saves
 // the atomics, but its pass does more per token: 155 us.
 // ---------------------------------------------------------------------------------------
 constexpr int kThreads = 512, kWarps = kThreads / 32;

@@ -198,8 +198,9 @@ def attention(q8, k_pages, v_pages, table, length, q_start, score_rq, out_rq, *,
     head_dim]` to the same shape (in `out` if given).
 
     `score_rq` = (Ms, Ss), `out_rq` = (Mo, So) and `prob_bits` are the graph's attention constants.
-    `max_rows` and `max_len` bound every sequence's new rows and its length: what is beyond them is
-    not computed.  Keys whose page id lies outside the cache count as absent; a row without keys
+    `max_rows` and `max_len` bound the new rows and the length of every sequence that has rows: what is
+    beyond them is not computed.  They also size the launch and choose its kernel, so bounds near the
+    true ones are faster.  Keys whose page id lies outside the cache count as absent; a row without keys
     gets zeros."""
     lib = _lib or _load()
     if out is None:
@@ -269,7 +270,8 @@ def reserve(table, length, refs, slots, counts, page_size, *, status=None) -> No
 
 
 def free(table, length, refs, slots, *, status=None) -> None:
-    """Gives the slots' pages back and sets their lengths to 0."""
+    """Gives the slots' pages back and sets their lengths to 0.  Slots outside the table are skipped and
+    noted in `status`, the others freed all the same."""
     _page_call("llx_pages_free", _no_pool(refs, 16), table, length, refs, slots, None, 0, None, None, status)
 
 
@@ -285,8 +287,8 @@ def fork(k_pages, v_pages, table, length, refs, parents, children, *, share=True
 
 
 def compact(k_pages, v_pages, table, refs, *, out=None, status=None):
-    """Moves the live pages (refs > 0) to the lowest ids, keeping their order, and renames them in
-    the table.  `out` = (table, refs) receives the renamed ones; default: in place.  Returns them."""
+    """Brings the live pages (refs > 0) to the lowest ids and renames them in the table: of n live pages
+    those with an id from n on move, in order, into the free ids below n, the others stay.  `out` = (table, refs) receives the renamed ones; default: in place.  Returns them."""
     new_table, new_refs = (table, refs) if out is None else out
     if new_table.shape != table.shape or new_table.stride() != table.stride():
         raise ValueError("the new table must be laid out like the table")
