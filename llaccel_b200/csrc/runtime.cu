@@ -863,6 +863,7 @@ struct PagedState {
   std::vector<int> len;             // host copy of the lengths
   std::vector<char> broken;         // slots that a failed call left half done: closed until they are freed
   bool damaged = false;             // a compaction failed half way: the tables are of no more use
+  bool unread = false;              // a call failed before it read what its kernels noted
   std::vector<int> q_norm, k_norm;  // per plan step: the norm steps its append takes over, or -1
   std::vector<char> skipped;        // per plan step: a norm that an append takes over
   int n = 0, rows = 0, max_rows = 0, max_len = 0;  // the launch under way
@@ -1944,15 +1945,25 @@ static void paged_accept(int32_t code) {
 // What a call does once it has begun to change slots.  LLX_ERR_OOM tells the caller that nothing was changed,
 // so it is not among the errors that come out of here.
 template <class F>
-static void paged_commit(F&& f) {
+static void paged_commit(llx_session* s, F&& f) {
+  s->paged->unread = true;
   try {
     f();
+    s->paged->unread = false;
   } catch (const Error& e) {
     if (e.code == LLX_ERR_OOM) throw Error(LLX_ERR_CUDA, e.what());
     throw;
   } catch (const std::bad_alloc&) {
     throw Error(LLX_ERR_CUDA, "host allocation failed");
   }
+}
+
+// what kernels of a call that failed have noted is not the next call's
+static void paged_begin(llx_session* s) {
+  if (!s->paged->unread) return;
+  LLX_CUDA(cudaMemsetAsync(s->paged->status, 0, sizeof(int32_t), s->st));
+  LLX_CUDA(cudaMemsetAsync(s->d_err, 0, 2 * sizeof(int32_t), s->st));
+  s->paged->unread = false;
 }
 
 static int paged_need(const PagedState& p, int len) { return (len + p.page_size - 1) / p.page_size; }
@@ -2550,6 +2561,7 @@ llx_status llx_serve_step(llx_serve* h, int n, const int32_t* slots, const int32
     const bool sampled = how && how->random;
     require(!sampled || m->vocab <= sample_max_vocab(), LLX_ERR_UNSUPPORTED, "the vocabulary is too large to sample from");
     cudaSetDevice(m->device);
+    paged_begin(s);
     if (logits) ensure_i16(s, (size_t)n * m->vocab_padded);
     stage_tokens(s, tokens, (int)rows);
     paged_put(s, p.slots, slots, n);
@@ -2562,7 +2574,7 @@ llx_status llx_serve_step(llx_serve* h, int n, const int32_t* slots, const int32
     paged_mark(p, n, slots, true);  // until the step is done
     for (int i = 0; i < n; ++i) p.len[slots[i]] += counts[i];
     bool full = false;
-    paged_commit([&] {
+    paged_commit(s, [&] {
       if (tight) {
         const int32_t code = paged_status(s);
         full = code & LLX_STATUS_NO_PAGES;
@@ -2634,6 +2646,7 @@ llx_status llx_serve_fork(llx_serve* h, int n, const int32_t* parents, const int
     for (int i = 0; i < n; ++i)
       require(!is_child[parents[i]], LLX_ERR_INVALID, "slot " + std::to_string(parents[i]) + " is both parent and child");
     cudaSetDevice(s->m->device);
+    paged_begin(s);
     paged_put(s, p.slots, parents, n);
     paged_put(s, p.counts, children, n);
     llx_pages_args a = paged_pages(s, n);
@@ -2643,7 +2656,7 @@ llx_status llx_serve_fork(llx_serve* h, int n, const int32_t* parents, const int
     paged_mark(p, n, children, true);  // until the call is done
     for (int i = 0; i < n; ++i) p.len[children[i]] = std::max(len[children[i]], len[parents[i]]);
     int32_t code = 0;
-    paged_commit([&] {
+    paged_commit(s, [&] {
       LLX_CUDA(launch_pages_fork(a, s->st));
       code = paged_status(s);
     });
@@ -2684,7 +2697,7 @@ llx_status llx_serve_compact(llx_serve* h) {
     a.new_table = p.table;
     a.new_refs = p.refs;
     p.damaged = true;  // until the call is done
-    paged_commit([&] {
+    paged_commit(s, [&] {
       LLX_CUDA(launch_pages_compact(a, s->st));
       LLX_CUDA(cudaStreamSynchronize(s->st));
     });

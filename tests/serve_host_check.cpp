@@ -12,7 +12,7 @@
 static int ops = 0, fail_at = 0;  // operations of the call under test; the one that fails (0: none)
 static cudaError_t fail_with = cudaSuccess;
 static bool reserved;  // the call under test has begun to change slots
-static bool no_pages, bad_page;
+static bool no_pages, bad_page, lost;
 
 static cudaError_t tick() { return ++ops == fail_at ? fail_with : cudaSuccess; }
 
@@ -56,6 +56,7 @@ int sab_rows_per_tile(int) { return 64; }
 cudaError_t launch_pages_reserve(const llx_pages_args& a, cudaStream_t) {
   const cudaError_t e = tick();
   if (e != cudaSuccess) return e;
+  if (lost) *a.status |= LLX_STATUS_LOST;
   if (no_pages)
     *a.status |= LLX_STATUS_NO_PAGES;
   else
@@ -206,6 +207,23 @@ static void compactions(llx_model* m, cudaError_t e) {
   }
 }
 
+// what a failed step's kernels have noted is its own: the calls after it neither fail by it nor take it for
+// a refusal of theirs
+static void notes(llx_model* m) {
+  for (int fork = 0; fork < 2; ++fork)
+    for (int n = 1; n < 60; ++n) {
+      Serve s(m);
+      CHECK(s.step({0, 2}) == LLX_OK);
+      lost = true;
+      CHECK(failing(n, cudaErrorLaunchOutOfResources, [&] { return s.step({0, 1}); }) != LLX_OK);
+      lost = false;
+      if (fork)
+        CHECK(s.fork({2}, {3}) == LLX_OK && s.len(3) == 3 && s.step({3}) == LLX_OK);
+      else
+        CHECK(s.step({2}) == LLX_OK && s.len(2) == 6);
+    }
+}
+
 // a buffer that could not be made larger is not taken for the one it was
 static void logits_buffer(llx_model* m) {
   for (int n = 1; n < 5; ++n) {
@@ -227,6 +245,7 @@ int main(int argc, char** argv) {
   }
   too_few_pages(m);
   logits_buffer(m);
+  notes(m);
   llx_model_destroy(m);
   printf("%d failures\n", failures);
   return failures != 0;
